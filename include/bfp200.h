@@ -307,6 +307,94 @@ int bfp200_fwd_layer_decode(bfp200_handle* h, int layer, const double* h_in, con
                             const int32_t* kv_pos, int ncols, double* k_cache, double* v_cache, int max_ctx,
                             double* h_out, double* stages);
 
+/* ---- rotary positions and a paged KV cache held in 4 bits -----------------
+ * No counterpart in the reference, whose cache is 16-bit BFP.  Operators on
+ * DEVICE memory of the current device, asynchronous on `stream` (a
+ * cudaStream_t, NULL for the default stream); they allocate nothing, keep
+ * nothing between calls and may be captured into a graph.  Arguments that a
+ * host check can see to be wrong give BFP200_EINVAL before anything runs.
+ * Strides are in elements; the last axis (head dim) is contiguous.
+ *
+ * The cache holds BFP tiles of 16 head dims with 4-bit mantissas:
+ *   e = clip(floor(log2(max|v|)) + 1, -17, 12), m = clip(rint(v 2^(3-e)), -8, 7)
+ * as nibble m + 8 and byte e + 18; |v| > 3584 saturates, NaN becomes 0.  One
+ * record of page * HD * 9 / 8 bytes per (page, KV head):
+ *   keys   [page/4][HD/8][4 positions][4 B]  nibble n of a word: dim 8 u + n
+ *   values [page/8][HD/4][4 i][2 h][2 B]     position 8 o + 4 h + i, nibble n: dim 4 u + n
+ *   key exponents [HD/16][page], value exponents [HD/16][page]
+ *
+ * A batch: sequence s has lens[s] positions in the pages block_table[s][0..],
+ * of which the last q_start[s+1] - q_start[s] are this call's tokens (rows
+ * q_start[s].. of the [n_tokens] arrays).  These arrays are read on the
+ * device: q_start ascends from 0 to n_tokens.  Values that do not fit are
+ * never followed out of bounds: a token without a position (negative, past
+ * max_pages * page, outside q_start) or whose table entry is no page of the
+ * pool is not written, and reads as zeros. */
+enum { BFP200_F32 = 0, BFP200_F16 = 1, BFP200_BF16 = 2 };
+
+typedef struct bfp200_rope_args {
+  const void* x_dev;                      /* [T][H][HD] */
+  void* out_dev;                          /* [T][H][HD]; may be x_dev */
+  const float* table_dev;                 /* [n_pos][rot/2][2]: cos, sin */
+  const int32_t* positions_dev;           /* [T]; outside 0..n_pos-1: the nearest */
+  long long x_ts, x_hs, o_ts, o_hs;       /* token and head strides of x and out */
+  long long T, H, HD, n_pos, rot;         /* rot: leading dims that are rotated (even) */
+  long long dtype, interleaved, inverse;  /* pairs (2j, 2j+1) or (j, j + rot/2); inverse: the gradient */
+} bfp200_rope_args;
+/* out = x with the pairs of its first rot dims turned by their position's
+ * angles, the rest copied; each product and sum rounded once in 32 bits. */
+int bfp200_rope_dev(const bfp200_rope_args* args, void* stream);
+
+typedef struct bfp200_kv4_batch {
+  void* pool_dev;                         /* [n_pages][H_KV][page * HD * 9 / 8], 16-byte aligned */
+  const int32_t* block_table_dev;         /* [n_seq][table_stride] */
+  const int32_t* q_start_dev;             /* [n_seq + 1] */
+  const int32_t* lens_dev;                /* [n_seq] */
+  long long n_pages, page, H_KV, HD;      /* page 16, 32, 64, 128 or 256; HD 32, 64, 96 or 128 */
+  long long n_seq, max_pages, table_stride, n_tokens;
+} bfp200_kv4_batch;
+
+typedef struct bfp200_kv4_append_args {
+  bfp200_kv4_batch batch;
+  const void *k_dev, *v_dev, *q_dev;      /* [n_tokens][H_KV | H_KV | H_Q][HD] */
+  void* q_out_dev;                        /* rotated queries; may be q_dev */
+  long long k_ts, k_hs, v_ts, v_hs, q_ts, q_hs, o_ts, o_hs;
+  const float* table_dev;                 /* [n_pos][rot/2][2], or NULL: no rotation */
+  const int32_t* positions_dev;           /* [n_tokens] rotation positions, or NULL: the cache positions */
+  long long H_Q, n_pos, rot, dtype, interleaved;   /* H_Q 0: no queries */
+} bfp200_kv4_append_args;
+/* Rotates the call's keys and queries, quantizes keys and values and writes
+ * them to their pages. */
+int bfp200_kv4_append_dev(const bfp200_kv4_append_args* args, void* stream);
+
+typedef struct bfp200_kv4_read_args {
+  bfp200_kv4_batch batch;
+  void *k_out_dev, *v_out_dev;            /* [n_tokens][H_KV][HD], contiguous, 16-byte aligned */
+  long long dtype;
+} bfp200_kv4_read_args;
+/* The values that the cache holds for the call's tokens (exact in every dtype). */
+int bfp200_kv4_read_dev(const bfp200_kv4_read_args* args, void* stream);
+
+typedef struct bfp200_kv4_attention_args {
+  bfp200_kv4_batch batch;
+  const void* q_dev;                      /* [n_tokens][H_Q][HD] */
+  void* out_dev;                          /* [n_tokens][H_Q][HD] */
+  float* lse_dev;                         /* [n_tokens][H_Q] log-sum-exp of the scaled scores, or NULL */
+  void* workspace_dev;                    /* 16-byte aligned; contents do not matter */
+  long long workspace_bytes;
+  long long q_ts, q_hs, o_ts, o_hs;
+  long long H_Q, dtype, causal, window;   /* H_Q a multiple of H_KV; window 0: none */
+  double scale;
+} bfp200_kv4_attention_args;
+/* Softmax attention of the call's tokens over their sequences' cached
+ * positions.  A token at position p sees the positions k < lens[s] with k <= p
+ * (causal) and k > p - window (window > 0); one that sees none gives zeros and
+ * -inf. */
+int bfp200_kv4_attention_dev(const bfp200_kv4_attention_args* args, void* stream);
+/* Bytes of workspace that a call with this head dim needs, whatever its other
+ * sizes (some 20 MB at most). */
+int bfp200_kv4_attention_workspace(const bfp200_kv4_attention_args* args, size_t* bytes);
+
 /* Stage dump layout of bfp200_fwd_layer (mirrors the N1..D dumps of
  * gen_smollm_blockfp_bfp.py:393-426): n1 q k v attn o h1 n2 g u mlp d, where
  * n1/n2/attn/mlp are the matvec inputs tile_quantize(.) decoded, q/k are

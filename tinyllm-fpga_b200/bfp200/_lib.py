@@ -77,6 +77,11 @@ SIGNATURES = {
     "bfp200_head_shard": [_P, _P, _I, _I],
     "bfp200_head_shard_group": [_P, _I],
     "bfp200_generate_sharded": [_P, _I, _P, _P, _I, _I, _I, _P],
+    "bfp200_rope_dev": [_P, _P],
+    "bfp200_kv4_append_dev": [_P, _P],
+    "bfp200_kv4_read_dev": [_P, _P],
+    "bfp200_kv4_attention_dev": [_P, _P],
+    "bfp200_kv4_attention_workspace": [_P, C.POINTER(_Z)],
 }
 NCCL_ID_BYTES = 128
 
