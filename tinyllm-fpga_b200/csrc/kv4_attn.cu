@@ -27,6 +27,7 @@
 // partial sums that a second, dependent launch joins in a fixed order.
 #include "kv4.cuh"
 
+#include <cmath>
 #include <exception>
 #include <string>
 #include <type_traits>
@@ -37,11 +38,26 @@ namespace bfp {
 namespace kv4 {
 namespace {
 
-constexpr int BLK = 32;            // positions of one step of a warp
+// Positions of one step of a warp: 32-position tiles of the tensor-core
+// operands, two of them where the head dim leaves room, so that a step's fixed
+// work (addresses, waits, the test of the maximum) is shared by more values.
+template <int HD> constexpr int SUB = HD <= 64 ? 2 : 1;
+template <int HD> constexpr int BLK_OF = 32 * SUB<HD>;
 constexpr int MINB = 8;            // blocks that are not worth a second CTA
 constexpr float LN2 = 0.6931471805599453f;
-constexpr float P_EXP = 15.f;      // P is held times 2^15: subnormal only below 2^-29 of the maximum
+// P is held times 2^P_EXP, at most 2^(P_EXP + SLACK) = 2^15: with one binary16
+// operand it turns subnormal (errors of 2^-32 of the maximum's weight) below
+// 2^-21, with two below 2^-28.
+template <int PS> constexpr float P_EXP = PS == 1 ? 7.f : 14.f;
+template <int PS> constexpr float SLACK = PS == 1 ? 8.f : 1.f;
 constexpr float V_UP = 16.f;       // V is held times 2^-4
+
+// An item cut over CTAs c .. c + parts - 1, left by CTA c for the joining launch.
+struct Cut {
+  int parts;                       // 0: none
+  int q0, rows, r0, head0;         // first token, rows, first row, first query head
+  int pad[3];
+};
 
 struct AttnArgs {
   Batch b;
@@ -49,10 +65,13 @@ struct AttnArgs {
   void* out;
   float* lse;                      // [T][HQ] or null
   float* part;                     // partial sums: [CTA][2][NR][HD + 2]
+  Cut* cuts;                       // [CTA]: the item that the CTA begins and does not end
   long long q_ts, q_hs, o_ts, o_hs;
   int HQ, group, causal;
   long long window;                // 0: none
-  float scale_log2;
+  float scale_log2;                // > 0: a negative scale negates the queries
+  float slack[2];                  // SLACK<1>, SLACK<2> in units of the scores
+  unsigned q_flip;                 // sign bits to flip in a pair of 16-bit queries
   int grid;                        // CTAs of the first launch
 };
 
@@ -61,70 +80,86 @@ struct Seq {
   int q0, n_q, len, blk0, nb, rt;  // first token, tokens, positions, first block, blocks, row tiles
 };
 
-template <int NR>
-__device__ __forceinline__ Seq seq_of(const AttnArgs& a, int s) {
-  Seq r;
-  const int qs = min(max(__ldg(a.b.q_start + s), 0), a.b.T);
-  const int qe = min(max(__ldg(a.b.q_start + s + 1), qs), a.b.T);
-  r.q0 = qs;
-  r.n_q = qe - qs;
-  r.len = min(max(__ldg(a.b.lens + s), 0), a.b.max_pages << a.b.page_shift);
-  const long long first = a.window ? (long long)r.len - r.n_q - a.window + 1 : 0;
-  r.blk0 = first > 0 ? min((int)(first / BLK), max(r.len - 1, 0) / BLK) : 0;
-  r.nb = max((r.len + BLK - 1) / BLK - r.blk0, 1);
-  r.rt = (int)(((long long)r.n_q * a.group + NR - 1) / NR);
-  return r;
-}
-
-constexpr int SCH = 128;           // chunks of sequences whose block counts are summed
+// Blocks before each sequence (or chunk of `per` sequences, where there are
+// more than SCH), summed by every CTA for itself.
+constexpr int SCH = 256;
 struct Sched {
-  long long pre[SCH + 1];          // blocks before each chunk
+  long long pre[SCH + 1];
   long long total, geff, delta;
-  int per;                         // sequences per chunk
+  int q0[SCH], n_q[SCH], len[SCH];   // the sequences themselves, where per == 1
+  long long wsum[16], wit[16];
+  int per;
 };
 
+// What follows from a sequence's first token, tokens and length.
+template <int NR, int BLK>
+__device__ __forceinline__ Seq seq_make(const AttnArgs& a, int q0, int n_q, int len) {
+  Seq r;
+  r.q0 = q0;
+  r.n_q = n_q;
+  r.len = len;
+  const long long first = a.window ? (long long)len - n_q - a.window + 1 : 0;
+  r.blk0 = first > 0 ? min((int)(first / BLK), max(len - 1, 0) / BLK) : 0;
+  r.nb = max((len + BLK - 1) / BLK - r.blk0, 1);
+  const long long rows = (long long)n_q * a.group;
+  r.rt = (int)((rows + NR - 1) / NR);
+  return r;
+}
+template <int NR, int BLK>
+__device__ __forceinline__ Seq seq_of(const AttnArgs& a, int s) {
+  const int qs = min(max(__ldg(a.b.q_start + s), 0), a.b.T);
+  const int qe = min(max(__ldg(a.b.q_start + s + 1), qs), a.b.T);
+  return seq_make<NR, BLK>(a, qs, qe - qs, min(max(__ldg(a.b.lens + s), 0), a.b.max_pages << a.b.page_shift));
+}
+
 // Fills the schedule; every thread of the CTA takes part.
-template <int NR>
-__device__ void make_sched(const AttnArgs& a, Sched& s, int n_thr) {
-  __shared__ long long s_items;
-  const int per = (a.b.n_seq + SCH - 1) / SCH;
-  if (threadIdx.x == 0) s_items = 0;
-  __syncthreads();
-  long long items = 0;
-  for (int c = threadIdx.x; c < SCH; c += n_thr) {
-    long long w = 0;
+template <int NR, int BLK, int THR>
+__device__ void make_sched(const AttnArgs& a, Sched& s) {
+  constexpr int C = (SCH + THR - 1) / THR;                  // chunks of a thread
+  const int per = (a.b.n_seq + SCH - 1) / SCH, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long w[C] = {}, sum = 0, items = 0;
+  #pragma unroll
+  for (int k = 0; k < C; ++k) {
+    const int c = threadIdx.x * C + k;
+    w[k] = 0;
+    if (c >= SCH) break;
     for (int i = c * per; i < min((c + 1) * per, a.b.n_seq); ++i) {
-      const Seq q = seq_of<NR>(a, i);
+      const Seq q = seq_of<NR, BLK>(a, i);
+      if (per == 1) { s.q0[c] = q.q0; s.n_q[c] = q.n_q; s.len[c] = q.len; }
       const long long n = (long long)q.rt * a.b.H;
       items += n;
-      w += n * q.nb;
+      w[k] += n * q.nb;
     }
-    s.pre[c + 1] = w;
+    sum += w[k];
   }
-  for (int o = 16; o; o >>= 1) items += __shfl_xor_sync(0xffffffffu, items, o);
-  if ((threadIdx.x & 31) == 0 && items) atomicAdd(reinterpret_cast<unsigned long long*>(&s_items), (unsigned long long)items);
+  long long inc = sum;
+  #pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, inc, o), z = __shfl_xor_sync(0xffffffffu, items, o);
+    if (lane >= o) inc += y;
+    items += z;
+  }
+  if (lane == 31) { s.wsum[warp] = inc; s.wit[warp] = items; }
   __syncthreads();
-  if (threadIdx.x < 32) {                                   // inclusive sums: 4 chunks a lane
-    constexpr int C = SCH / 32;
-    long long v[C], sum = 0;
-    #pragma unroll
-    for (int i = 0; i < C; ++i) { sum += s.pre[threadIdx.x * C + i + 1]; v[i] = sum; }
-    long long inc = sum;
-    #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, inc, o);
-      if ((int)threadIdx.x >= o) inc += y;
-    }
-    #pragma unroll
-    for (int i = 0; i < C; ++i) s.pre[threadIdx.x * C + i + 1] = inc - sum + v[i];
-    if (threadIdx.x == 31) {
-      s.total = inc;
-      const long long want = max((long long)s_items, (inc + MINB - 1) / MINB);
-      s.geff = max(min((long long)a.grid, want), 1LL);
-      s.delta = max(inc / s.geff / 4, (long long)(MINB / 2));
-      s.pre[0] = 0;
-      s.per = per;
-    }
+  long long before = 0, total = 0, n_items = 0;
+  #pragma unroll
+  for (int k = 0; k < THR / 32; ++k) {
+    if (k < warp) before += s.wsum[k];
+    total += s.wsum[k];
+    n_items += s.wit[k];
+  }
+  long long at = before + inc - sum;
+  #pragma unroll
+  for (int k = 0; k < C; ++k) {
+    if (threadIdx.x * C + k < SCH) s.pre[threadIdx.x * C + k] = at;
+    at += w[k];
+  }
+  if (threadIdx.x == 0) {
+    s.pre[SCH] = total;
+    s.total = total;
+    s.geff = max(min((long long)a.grid, max(n_items, (total + MINB - 1) / MINB)), 1LL);
+    s.delta = max(total / (s.geff * 32), (long long)(MINB / 2));
+    s.per = per;
   }
   __syncthreads();
 }
@@ -135,35 +170,46 @@ struct Item {
   Seq q;
 };
 
+__device__ __forceinline__ long long div_small(long long x, long long y) {   // 32-bit where it fits: a third of the time
+  return ((x | y) >> 32) == 0 ? (long long)((unsigned)x / (unsigned)y) : x / y;
+}
+
 // The item that holds block x (0 <= x < total).
-template <int NR>
+template <int NR, int BLK>
 __device__ Item item_at(const AttnArgs& a, const Sched& s, long long x) {
   int lo = 0, hi = SCH;                                     // pre[lo] <= x < pre[hi]
+  #pragma unroll 1
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (s.pre[mid] <= x) lo = mid; else hi = mid;
   }
   Item it;
   long long at = s.pre[lo];
-  it.seq = lo * s.per;
-  for (;; ++it.seq) {
-    it.q = seq_of<NR>(a, it.seq);
-    const long long w = (long long)it.q.rt * a.b.H * it.q.nb;
-    if (x < at + w || it.seq + 1 >= a.b.n_seq) break;
-    at += w;
+  if (s.per == 1) {
+    it.seq = lo;
+    it.q = seq_make<NR, BLK>(a, s.q0[lo], s.n_q[lo], s.len[lo]);
+  } else {
+    it.seq = lo * s.per;
+    #pragma unroll 1
+    for (;; ++it.seq) {
+      it.q = seq_of<NR, BLK>(a, it.seq);
+      const long long w = (long long)it.q.rt * a.b.H * it.q.nb;
+      if (x < at + w || it.seq + 1 >= a.b.n_seq) break;
+      at += w;
+    }
   }
-  it.idx = (int)((x - at) / it.q.nb);
+  it.idx = (int)div_small(x - at, it.q.nb);
   it.start = at + (long long)it.idx * it.q.nb;
   it.end = it.start + it.q.nb;
   return it;
 }
 
 // First block of CTA i: an even share, moved onto an item's edge if one is near.
-template <int NR>
+template <int NR, int BLK>
 __device__ long long bound(const AttnArgs& a, const Sched& s, long long i) {
-  const long long x = i * s.total / s.geff;
+  const long long x = div_small(i * s.total, s.geff);
   if (x <= 0 || x >= s.total) return x <= 0 ? 0 : s.total;
-  const Item it = item_at<NR>(a, s, x);
+  const Item it = item_at<NR, BLK>(a, s, x);
   const long long before = x - it.start, after = it.end - x;
   if (before <= after) return before <= s.delta ? it.start : x;
   return after <= s.delta ? it.end : x;
@@ -171,18 +217,18 @@ __device__ long long bound(const AttnArgs& a, const Sched& s, long long i) {
 
 // ---- arithmetic ------------------------------------------------------------------
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const unsigned (&a)[4], uint2 b) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const unsigned (&a)[4], uint2 b) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 __device__ __forceinline__ unsigned transpose8(unsigned x) {
   unsigned y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -202,11 +248,20 @@ __device__ __forceinline__ unsigned prmt(unsigned a, unsigned b, unsigned sel) {
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(y) : "r"(a), "r"(b), "r"(sel));
   return y;
 }
-// (x & mask) | magic in one instruction
-template <unsigned MASK, unsigned MAGIC>
-__device__ __forceinline__ unsigned and_or(unsigned x) {
+// (x & MASK) | magic in one instruction, which takes one immediate: the magic
+// numbers stay in registers.
+struct Magic { unsigned h1024, h64, b128; };
+__device__ __forceinline__ Magic magic_numbers() {
+  Magic m;
+  asm volatile("mov.u32 %0, 0x64006400;" : "=r"(m.h1024));
+  asm volatile("mov.u32 %0, 0x54005400;" : "=r"(m.h64));
+  asm volatile("mov.u32 %0, 0x43004300;" : "=r"(m.b128));
+  return m;
+}
+template <unsigned MASK>
+__device__ __forceinline__ unsigned and_or(unsigned x, unsigned magic) {
   unsigned y;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "n"(MASK), "n"(MAGIC));
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "n"(MASK), "r"(magic));
   return y;
 }
 
@@ -223,11 +278,13 @@ __device__ __forceinline__ ScaleH scale_h(unsigned bytes) {       // exponent by
   r.c64 = as_u(__hmul2(h, __floats2half2_rn(-72.f * 0x1p-10f, -72.f * 0x1p-10f)));
   return r;
 }
-template <int N>
-__device__ __forceinline__ unsigned pair_h(unsigned w, unsigned w8, const ScaleH& sc) {   // w8 = w >> 8
-  const unsigned src = N < 2 ? w : w8;
-  const unsigned x = (N & 1) ? and_or<0x00F000F0u, 0x54005400u>(src) : and_or<0x000F000Fu, 0x64006400u>(src);
-  return as_u(__hfma2(as_h2(x), as_h2(sc.s), as_h2((N & 1) ? sc.c64 : sc.c1024)));
+__device__ __forceinline__ void pairs_h(const Magic& mg, unsigned w, const ScaleH& sc, unsigned (&o)[4]) {
+  const unsigned w8 = w >> 8;
+  const __half2 s = as_h2(sc.s), c0 = as_h2(sc.c1024), c1 = as_h2(sc.c64);
+  o[0] = as_u(__hfma2(as_h2(and_or<0x000F000Fu>(w, mg.h1024)), s, c0));
+  o[1] = as_u(__hfma2(as_h2(and_or<0x00F000F0u>(w, mg.h64)), s, c1));
+  o[2] = as_u(__hfma2(as_h2(and_or<0x000F000Fu>(w8, mg.h1024)), s, c0));
+  o[3] = as_u(__hfma2(as_h2(and_or<0x00F000F0u>(w8, mg.h64)), s, c1));
 }
 // Bfloat16 pairs: 128 + nibble, less 136, scaled; exact.
 struct ScaleB { unsigned s, c; };
@@ -237,10 +294,18 @@ __device__ __forceinline__ ScaleB scale_b(unsigned bytes) {
   r.c = as_u(__hmul2(as_b2(r.s), __floats2bfloat162_rn(-136.f, -136.f)));
   return r;
 }
-template <int N>
-__device__ __forceinline__ unsigned pair_b(unsigned w, const ScaleB& sc) {
-  const unsigned x = and_or<0x000F000Fu, 0x43004300u>(w >> (4 * N));
-  return as_u(__hfma2(as_b2(x), as_b2(sc.s), as_b2(sc.c)));
+__device__ __forceinline__ void pairs_b(const Magic& mg, unsigned w, const ScaleB& sc, unsigned (&o)[4]) {
+  #pragma unroll
+  for (int n = 0; n < 4; ++n) o[n] = as_u(__hfma2(as_b2(and_or<0x000F000Fu>(w >> (4 * n), mg.b128)), as_b2(sc.s), as_b2(sc.c)));
+}
+template <bool HALF> using KeyScaleT = std::conditional_t<HALF, ScaleH, ScaleB>;
+template <bool HALF> __device__ __forceinline__ KeyScaleT<HALF> key_scale(unsigned bytes) {
+  if constexpr (HALF) return scale_h(bytes);
+  else return scale_b(bytes);
+}
+template <bool HALF> __device__ __forceinline__ void key_pairs(const Magic& mg, unsigned w, const KeyScaleT<HALF>& sc, unsigned (&o)[4]) {
+  if constexpr (HALF) pairs_h(mg, w, sc, o);
+  else pairs_b(mg, w, sc, o);
 }
 
 template <typename T> struct Kind;
@@ -268,43 +333,87 @@ __device__ __forceinline__ void split_q(T a, T b, unsigned (&o)[Kind<T>::QS]) {
   }
 }
 
+// A warp's ring of 32-position tiles in shared memory, filled by cp.async with
+// consecutive 16-byte units per lane (a lane's own operand bytes lie 64 bytes
+// apart: fetched directly, every 32-byte sector would cross L2 twice).  A
+// unit's place is its index with low bits exchanged, so that the operand
+// reads, 8 lanes at a time, meet 8 different bank groups.
 template <int HD>
-struct Tile {                        // this lane's part of 32 positions
-  static constexpr int KU = HD / 32;
+struct Ring {
+  static constexpr int KU = HD / 32;                      // 16-byte units of a lane: keys, and values
   static constexpr int NKE = KU % 2 == 0 ? KU / 2 : KU;   // distinct exponent tiles of the lane's key units
   static constexpr int NVE = KU == 3 ? 3 : 1;             // ... of its value units
-  uint4 k[KU], v[KU];
-  unsigned ke[NKE];
-  uint2 ve[NVE];
+  static constexpr int KES = HD == 128 ? 48 : 32, VES = 32;      // bytes between the exponents of two tiles
+  static constexpr int KE = HD * 16, KB1 = KE + HD / 16 * KES, VE = HD * 16, VB1 = VE + HD / 16 * VES;
+  static constexpr int KB = SUB<HD> * KB1, VB = SUB<HD> * VB1;   // bytes of a stage of keys, of values
+  // key unit (quad g, unit t KU + w), value unit (oct t, unit g KU + w)
+  __device__ static __forceinline__ int k_place(int u) {
+    return HD == 128 ? u ^ (u >> 2 & 3) ^ (u >> 4 & 1) << 2 : HD == 64 ? u ^ (u >> 3 & 1) : u;
+  }
+  __device__ static __forceinline__ int v_place(int u) {
+    return HD == 128 ? u ^ (u >> 5 & 3) : HD == 64 ? u ^ (u >> 4 & 1) ^ (u >> 5 & 1) << 2
+         : HD == 32 ? u ^ (u >> 3 & 3) << 1 : u ^ (u / 24 & 3) << 1;
+  }
+  // place(32 i + lane) * 16 - place(lane) * 16, given an address that holds place(lane) and is a multiple of 128 else
+  __device__ static __forceinline__ int k_move(int i, unsigned at) { return i * 512; }
+  __device__ static __forceinline__ int v_move(int i, unsigned at) {
+    const int x = HD == 128 ? i : HD == 64 ? i << 2 : 0;
+    if (HD == 96) {
+      const int l = threadIdx.x & 31;
+      return (v_place(32 * i + l) - v_place(l)) * 16;
+    }
+    return i * 512 + (int)((at ^ (x << 4)) - at);
+  }
 };
-
-__device__ __forceinline__ uint4 ld16(const uint8_t* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
+__device__ __forceinline__ unsigned su32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(unsigned d, const void* g) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(d), "l"(g) : "memory");
 }
 
-template <typename T, int HD, int NT, int W>
-__global__ void __launch_bounds__(W * 32) attn_kernel(const AttnArgs a) {
+// Launch shape by row tiles: warps, CTAs of an SM, stages of a warp's ring.
+// CTAs of 4 warps rather than 8: one's start and joining run beside another's
+// loop.  Registers set their number: 128 at HD <= 64, 168 above (64 sequences
+// of 4608 positions, 32 / 8 heads of 128: 3 x 4 warps 91 us, 2 x 6 98 us, 1 x 12
+// 97 us, 2 x 8 at 128 registers 107 us; 37 of 8192, 24 / 8 heads of 64: 4 x 4
+// warps 55 us, 3 x 8 at 80 registers 69 us).
+template <int HD, int NT> struct Shape {
+  static constexpr int W = 4, CTAS = NT == 1 ? (HD <= 64 ? 4 : 3) : NT == 2 && HD <= 64 ? 3 : 2;
+  static constexpr int STAGES = HD == 128 || HD == 64 ? 2 : 3;   // of keys; values have one more
+  static constexpr int NR = NT * 8;
+  static constexpr int RING = W * (STAGES * Ring<HD>::KB + (STAGES + 1) * Ring<HD>::VB), MERGE = W * NR * (HD + 2) * 4;
+  template <int QS> static constexpr size_t smem() {
+    return (size_t)(HD / 16) * NT * QS * 32 * 8 + (RING > MERGE ? RING : MERGE);
+  }
+};
+
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(Shape<HD, NT>::W * 32, Shape<HD, NT>::CTAS) attn_kernel(const AttnArgs a) {
+  using SH = Shape<HD, NT>;
+  using RG = Ring<HD>;
+  constexpr int W = SH::W, STAGES = SH::STAGES, SB = SUB<HD>, BLK = BLK_OF<HD>;
   constexpr int NR = NT * 8, KU = HD / 32, QS = Kind<T>::QS, PS = Kind<T>::PS, REC9 = HD * 9 / 8;
   constexpr bool HALF_K = Kind<T>::HALF_K;
-  using TL = Tile<HD>;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   uint2* s_q = reinterpret_cast<uint2*>(smem);                        // [HD/16][NT][QS][32]
-  float* s_o = reinterpret_cast<float*>(s_q + HD / 16 * NT * QS * 32);  // [W][NR][HD]
+  unsigned char* k_ring = smem + HD / 16 * NT * QS * 32 * 8 + (threadIdx.x >> 5) * (SH::RING / W);
+  unsigned char* v_ring = k_ring + STAGES * RG::KB;
+  float* s_o = reinterpret_cast<float*>(s_q + HD / 16 * NT * QS * 32);  // after the loop, over the rings: [W][NR][HD]
   float* s_m = s_o + W * NR * HD;                                     // [W][NR], [W][NR]
   float* s_l = s_m + W * NR;
   __shared__ Sched sch;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  make_sched<NR>(a, sch, W * 32);
+  make_sched<NR, BLK, W * 32>(a, sch);
+  if (tid == 0) a.cuts[blockIdx.x].parts = 0;
   if ((long long)blockIdx.x >= sch.geff || sch.total == 0) return;
-  long long x = bound<NR>(a, sch, blockIdx.x);
-  const long long x1 = bound<NR>(a, sch, (long long)blockIdx.x + 1);
+  long long x = bound<NR, BLK>(a, sch, (long long)blockIdx.x + (lane & 1));   // both bounds at once
+  const long long x1 = __shfl_sync(0xffffffffu, x, 1);
+  x = __shfl_sync(0xffffffffu, x, 0);
   const int page = a.b.page, rec_bytes = page * REC9;
+  const long long page_bytes = (long long)rec_bytes * a.b.H;
+  const Magic mg = magic_numbers();
   Item it;
-  if (x < x1) it = item_at<NR>(a, sch, x);
+  if (x < x1) it = item_at<NR, BLK>(a, sch, x);
   while (x < x1) {
     const long long xe = min(x1, it.end);
     if (xe <= x) break;                                               // lengths changed during the call
@@ -327,7 +436,7 @@ __global__ void __launch_bounds__(W * 32) attn_kernel(const AttnArgs a) {
         for (int k = 0; k < QS; ++k) o0[k] = o1[k] = 0;
       }
       #pragma unroll
-      for (int k = 0; k < QS; ++k) s_q[((st * NT + nt) * QS + k) * 32 + l] = make_uint2(o0[k], o1[k]);
+      for (int k = 0; k < QS; ++k) s_q[((st * NT + nt) * QS + k) * 32 + l] = make_uint2(o0[k] ^ a.q_flip, o1[k] ^ a.q_flip);
     }
     // ---- what the rows see
     const int j0 = r0 / a.group, j1 = (r0 + rows - 1) / a.group;
@@ -343,10 +452,11 @@ __global__ void __launch_bounds__(W * 32) attn_kernel(const AttnArgs a) {
         hi[nt][c] = r < rows ? hi_of(j) : 0;
         lo[nt][c] = lo_of(j);
       }
-    float m[NT][2], lsum[NT][2], O[KU][2][NT][4];
+    float m[NT][2], ref[NT][2], lsum[NT][2], O[KU][2][NT][4];
     #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
+      ref[nt][0] = ref[nt][1] = 0.f;
       lsum[nt][0] = lsum[nt][1] = 0.f;
       #pragma unroll
       for (int w = 0; w < KU; ++w)
@@ -365,48 +475,78 @@ __global__ void __launch_bounds__(W * 32) attn_kernel(const AttnArgs a) {
       const int i = pos >> a.b.page_shift;
       return i < a.b.max_pages ? __ldg(bt + i) : -1;
     };
-    const auto load = [&](TL& tl, int base, int pk, int pv) {
-      const int slot_k = (base + 4 * g) & (page - 1), slot_v = (base + 8 * t) & (page - 1);
-      if ((unsigned)pk < (unsigned)a.b.n_pages) {
-        const uint8_t* rec = a.b.pool + ((long long)pk * a.b.H + h) * rec_bytes;
-        const uint8_t* kp = rec + ((slot_k >> 2) * (HD / 8) + t * KU) * 16;
+    const uint8_t* pool_h = a.b.pool + (long long)h * rec_bytes;
+    const bool one_page = page >= BLK;                                // a block lies in one page
+    const bool halves = page < 32;                                    // a tile's 32 positions lie in two pages
+    int pk[2 * SB];                                                   // pages of the next block to fetch
+    const auto pages = [&](int base) {
+      pk[0] = page_at(base);
+      if (!one_page) {
         #pragma unroll
-        for (int w = 0; w < KU; ++w) tl.k[w] = ld16(kp + w * 16);
-        #pragma unroll
-        for (int w = 0; w < TL::NKE; ++w) {
-          const int tile = TL::NKE == KU ? (t * KU + w) / 2 : t * TL::NKE + w;
-          tl.ke[w] = __ldg(reinterpret_cast<const unsigned*>(rec + page * HD + tile * page + slot_k));
-        }
-      } else {
-        #pragma unroll
-        for (int w = 0; w < KU; ++w) tl.k[w] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-        #pragma unroll
-        for (int w = 0; w < TL::NKE; ++w) tl.ke[w] = 0x01010101u;
+        for (int i = 1; i < 2 * SB; ++i) pk[i] = halves || i % 2 == 0 ? page_at(base + 16 * i) : pk[i - 1];
       }
-      if ((unsigned)pv < (unsigned)a.b.n_pages) {
-        const uint8_t* rec = a.b.pool + ((long long)pv * a.b.H + h) * rec_bytes;
-        const uint8_t* vp = rec + page * HD / 2 + ((slot_v >> 3) * (HD / 4) + g * KU) * 16;
+    };
+    const unsigned k_dst = su32(k_ring) + RG::k_place(lane) * 16, v_dst = su32(v_ring) + RG::v_place(lane) * 16;
+    const unsigned e_dst = lane < HD / 8 ? su32(k_ring) + RG::KE + (lane >> 1) * RG::KES + (lane & 1) * 16
+                                         : su32(v_ring) + RG::VE + ((lane >> 1) - HD / 16) * RG::VES + (lane & 1) * 16;
+    const int e_stage = lane < HD / 8 ? RG::KB1 : RG::VB1, e_src = page * HD + (lane >> 1) * page + (lane & 1) * 16 - lane * 16;
+    const auto load = [&](int ks, int vs, int base) {
+      if (one_page && (unsigned)pk[0] < (unsigned)a.b.n_pages) {
+        const uint8_t* src = pool_h + (long long)pk[0] * page_bytes + (base & (page - 1)) * (HD / 2) + lane * 16;
+        const uint8_t *vsrc = src + page * HD / 2, *esrc = src + (e_src - (base & (page - 1)) * (HD / 2 - 1));
+        const unsigned kd = k_dst + ks * RG::KB, vd = v_dst + vs * RG::VB, ed = e_dst + (lane < HD / 8 ? ks : vs) * SB * e_stage;
         #pragma unroll
-        for (int w = 0; w < KU; ++w) tl.v[w] = ld16(vp + w * 16);
-        #pragma unroll
-        for (int w = 0; w < TL::NVE; ++w) {
-          const int tile = (g * KU + w) / 4;
-          tl.ve[w] = __ldg(reinterpret_cast<const uint2*>(rec + page * HD + (HD / 16 + tile) * page + slot_v));
+        for (int sub = 0; sub < SB; ++sub) {                          // 32 positions on: 16 HD bytes of keys and of values
+          #pragma unroll
+          for (int i = 0; i < KU; ++i) {
+            cp16(kd + sub * RG::KB1 + RG::k_move(i, kd), src + sub * 16 * HD + i * 512);
+            cp16(vd + sub * RG::VB1 + RG::v_move(i, vd), vsrc + sub * 16 * HD + i * 512);
+          }
+          if (lane < HD / 4) cp16(ed + sub * e_stage, esrc + sub * 32);   // 32 bytes of every key and value tile
         }
-      } else {
+        return;
+      }
+      #pragma unroll 1
+      for (int i = 0; i < 2 * SB; ++i) {                              // 16 positions at a time; of no page: zeros
+        unsigned char *kst = k_ring + ks * RG::KB + (i >> 1) * RG::KB1, *vst = v_ring + vs * RG::VB + (i >> 1) * RG::VB1;
+        const int hf = i & 1, at = (base + 16 * i) & (page - 1);
+        int pg = pk[0];
         #pragma unroll
-        for (int w = 0; w < KU; ++w) tl.v[w] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+        for (int k = 1; k < 2 * SB; ++k) pg = !one_page && i == k ? pk[k] : pg;
+        const bool ok = (unsigned)pg < (unsigned)a.b.n_pages;
+        const uint8_t* rec = pool_h + (ok ? (long long)pg * page_bytes : 0);
+        const uint4 zero = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
         #pragma unroll
-        for (int w = 0; w < TL::NVE; ++w) tl.ve[w] = make_uint2(0x01010101u, 0x01010101u);
+        for (int u0 = 0; u0 < HD / 2; u0 += 32) {
+          const int u = u0 + lane;
+          if (u < HD / 2) {
+            unsigned char *kd = kst + RG::k_place(u + hf * (HD / 2)) * 16, *vd = vst + RG::v_place(u + hf * (HD / 2)) * 16;
+            const uint8_t* from = rec + at * (HD / 2) + u * 16;
+            if (ok) {
+              cp16(su32(kd), from);
+              cp16(su32(vd), from + page * HD / 2);
+            } else {
+              *reinterpret_cast<uint4*>(kd) = zero;
+              *reinterpret_cast<uint4*>(vd) = zero;
+            }
+          }
+        }
+        if (lane < HD / 8) {
+          unsigned char* d = (lane < HD / 16 ? kst + RG::KE + lane * RG::KES : vst + RG::VE + (lane - HD / 16) * RG::VES) + hf * 16;
+          if (ok) cp16(su32(d), rec + page * HD + lane * page + at);
+          else *reinterpret_cast<uint4*>(d) = make_uint4(0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u);
+        }
       }
     };
 
-    const auto compute = [&](const TL& tl, int base) {
-      // ---- S^T = K Q^T: tiles of rows (position 4 g, 4 g + 1) and (4 g + 2, 4 g + 3)
-      // (the query's low parts are summed apart: the tensor core cuts addends off at the sum's last bit)
-      float S[2][NT][4], S_low[QS > 1 ? 2 : 1][QS > 1 ? NT : 1][4];
+    // S^T = K Q^T: tiles of rows (position 4 g, 4 g + 1) and (4 g + 2, 4 g + 3).
+    // (The query's low parts are summed apart: the tensor core cuts addends off at the sum's last bit.)
+    float S[SB * 2][NT][4], S_low[QS > 1 ? SB * 2 : 1][QS > 1 ? NT : 1][4];
+    unsigned P[PS][SB * 4][NT];
+    const auto scores = [&](int ks) {
+      const unsigned char* st = k_ring + ks * RG::KB;
       #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < SB * 2; ++i)
         #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           #pragma unroll
@@ -414,86 +554,94 @@ __global__ void __launch_bounds__(W * 32) attn_kernel(const AttnArgs a) {
             S[i][nt][k] = 0.f;
             if constexpr (QS > 1) S_low[i][nt][k] = 0.f;
           }
-      const auto keys = [&](auto W_) {
-        constexpr int w = decltype(W_)::value;
-        const unsigned word[4] = {tl.k[w].x, tl.k[w].y, tl.k[w].z, tl.k[w].w};
-        const unsigned eb = tl.ke[TL::NKE == KU ? w : w / 2];
-        unsigned op[4][4];                                       // [position][pair]
+      constexpr int WPT = RG::NKE == KU ? 1 : 2;                  // units of one exponent tile
+      #pragma unroll
+      for (int sub = 0; sub < SB; ++sub) {
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const unsigned by = __byte_perm(eb, 0, 0x4040 | (i * 0x0101));
-          if constexpr (HALF_K) {
-            const ScaleH sc = scale_h(by);
-            const unsigned w8 = word[i] >> 8;
-            op[i][0] = pair_h<0>(word[i], w8, sc);
-            op[i][1] = pair_h<1>(word[i], w8, sc);
-            op[i][2] = pair_h<2>(word[i], w8, sc);
-            op[i][3] = pair_h<3>(word[i], w8, sc);
-          } else {
-            const ScaleB sc = scale_b(by);
-            op[i][0] = pair_b<0>(word[i], sc);
-            op[i][1] = pair_b<1>(word[i], sc);
-            op[i][2] = pair_b<2>(word[i], sc);
-            op[i][3] = pair_b<3>(word[i], sc);
+        for (int e = 0; e < RG::NKE; ++e) {
+          const unsigned eb = *reinterpret_cast<const unsigned*>(st + sub * RG::KB1 + RG::KE + (WPT == 1 ? (t * KU + e) / 2 : t * RG::NKE + e) * RG::KES + 4 * g);
+          KeyScaleT<HALF_K> sc[4];
+          #pragma unroll
+          for (int i = 0; i < 4; ++i) sc[i] = key_scale<HALF_K>(prmt(eb, 0u, i | 0x40 | i << 8 | 0x4000));
+          #pragma unroll
+          for (int w2 = 0; w2 < WPT; ++w2) {
+            const int w = e * WPT + w2;
+            const uint4 kv = *reinterpret_cast<const uint4*>(st + sub * RG::KB1 + RG::k_place(g * (HD / 8) + t * KU + w) * 16);
+            const unsigned word[4] = {kv.x, kv.y, kv.z, kv.w};
+            unsigned op[4][4];                                       // [position][pair]
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) key_pairs<HALF_K>(mg, word[i], sc[i], op[i]);
+            #pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+              #pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                #pragma unroll
+                for (int k = 0; k < QS; ++k) {
+                  const uint2 qb = s_q[(((w * 2 + hf) * NT + nt) * QS + k) * 32 + lane];
+                  #pragma unroll
+                  for (int i = 0; i < 2; ++i) {
+                    const unsigned fr[4] = {op[2 * i][2 * hf], op[2 * i + 1][2 * hf], op[2 * i][2 * hf + 1], op[2 * i + 1][2 * hf + 1]};
+                    if constexpr (HALF_K) mma_f16(S[sub * 2 + i][nt], fr, qb);
+                    else if (k == 0) mma_bf16(S[sub * 2 + i][nt], fr, qb);
+                    else mma_bf16(S_low[QS > 1 ? sub * 2 + i : 0][QS > 1 ? nt : 0], fr, qb);
+                  }
+                }
           }
         }
-        #pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-          #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            #pragma unroll
-            for (int k = 0; k < QS; ++k) {
-              const uint2 qb = s_q[(((w * 2 + hf) * NT + nt) * QS + k) * 32 + lane];
-              #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const unsigned fr[4] = {op[2 * i][2 * hf], op[2 * i + 1][2 * hf], op[2 * i][2 * hf + 1], op[2 * i + 1][2 * hf + 1]};
-                if constexpr (HALF_K) mma_f16(S[i][nt], fr, qb);
-                else if (k == 0) mma_bf16(S[i][nt], fr, qb);
-                else mma_bf16(S_low[QS > 1 ? i : 0][QS > 1 ? nt : 0], fr, qb);
-              }
-            }
-      };
-      keys(std::integral_constant<int, 0>{});
-      if constexpr (KU > 1) keys(std::integral_constant<int, 1>{});
-      if constexpr (KU > 2) keys(std::integral_constant<int, 2>{});
-      if constexpr (KU > 3) keys(std::integral_constant<int, 3>{});
-
-      // ---- running softmax
-      const bool whole = base + BLK <= all_hi && base >= all_lo;
-      unsigned P[PS][4][NT];
-      bool moved = false;
-      float al[NT][2];
+      }
+    };
+    // Running softmax, S^T to P^T.  The reference m of a row moves only when a score
+    // passes it by more than `slack` (in powers of two; P stays below 2^16).
+    const auto weights = [&](int base, bool whole) {
+      float top[NT][2];
+      bool passed = false;
       #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float top[2];
+      for (int nt = 0; nt < NT; ++nt)
         #pragma unroll
         for (int c = 0; c < 2; ++c) {
           #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < SB * 4; ++i) {
             float& s = S[i >> 1][nt][(i & 1) * 2 + c];
             if constexpr (QS > 1) s += S_low[i >> 1][nt][(i & 1) * 2 + c];
-            s *= a.scale_log2;
             if (!whole) {
-              const int p = base + 4 * g + i;
+              const int p = base + (i >> 2) * 32 + 4 * g + (i & 3);
               s = p < hi[nt][c] && p >= lo[nt][c] ? s : -INFINITY;
             }
           }
-          top[c] = fmaxf(fmaxf(S[0][nt][c], S[0][nt][2 + c]), fmaxf(S[1][nt][c], S[1][nt][2 + c]));
-          #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
-          const float mn = fmaxf(m[nt][c], top[c]);
-          const float ref = mn == -INFINITY ? 0.f : mn;
-          al[nt][c] = ex2(m[nt][c] - ref);
-          moved |= mn != m[nt][c];
-          m[nt][c] = mn;
-          top[c] = ref - P_EXP;
+          top[nt][c] = fmaxf(fmaxf(S[0][nt][c], S[0][nt][2 + c]), fmaxf(S[1][nt][c], S[1][nt][2 + c]));
+          if constexpr (SB > 1)
+            top[nt][c] = fmaxf(top[nt][c], fmaxf(fmaxf(S[2][nt][c], S[2][nt][2 + c]), fmaxf(S[3][nt][c], S[3][nt][2 + c])));
+          passed |= top[nt][c] > m[nt][c] + a.slack[PS - 1];
         }
-        float add[2] = {0.f, 0.f};
+      if (__any_sync(0xffffffffu, passed)) {
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p0 = ex2(S[i >> 1][nt][(i & 1) * 2] - top[0]), p1 = ex2(S[i >> 1][nt][(i & 1) * 2 + 1] - top[1]);
-          add[0] += p0;
-          add[1] += p1;
+        for (int nt = 0; nt < NT; ++nt)
+          #pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            #pragma unroll
+            for (int o = 4; o < 32; o <<= 1) top[nt][c] = fmaxf(top[nt][c], __shfl_xor_sync(0xffffffffu, top[nt][c], o));
+            const float mn = fmaxf(m[nt][c], top[nt][c]);
+            const float al = mn == -INFINITY ? 1.f : ex2((m[nt][c] - mn) * a.scale_log2);
+            m[nt][c] = mn;
+            ref[nt][c] = mn == -INFINITY ? 0.f : mn * a.scale_log2 - P_EXP<PS>;
+            lsum[nt][c] *= al;
+            #pragma unroll
+            for (int w = 0; w < KU; ++w)
+              #pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                O[w][n][nt][c] *= al;
+                O[w][n][nt][2 + c] *= al;
+              }
+          }
+      }
+      #pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        #pragma unroll
+        for (int i = 0; i < SB * 4; ++i) {
+          const float p0 = ex2(__fmaf_rn(S[i >> 1][nt][(i & 1) * 2], a.scale_log2, -ref[nt][0]));
+          const float p1 = ex2(__fmaf_rn(S[i >> 1][nt][(i & 1) * 2 + 1], a.scale_log2, -ref[nt][1]));
+          lsum[nt][0] += p0;
+          lsum[nt][1] += p1;
           const __half2 hp = __floats2half2_rn(p0, p1);
           P[0][i][nt] = transpose8(as_u(hp));
           if constexpr (PS == 2) {
@@ -501,78 +649,98 @@ __global__ void __launch_bounds__(W * 32) attn_kernel(const AttnArgs a) {
             P[1][i][nt] = transpose8(as_u(__floats2half2_rn(p0 - back.x, p1 - back.y)));
           }
         }
-        lsum[nt][0] = lsum[nt][0] * al[nt][0] + add[0];
-        lsum[nt][1] = lsum[nt][1] * al[nt][1] + add[1];
-      }
-      if (__any_sync(0xffffffffu, moved)) {
+    };
+    // O^T += V^T P^T
+    const auto accumulate = [&](int vs) {
+      #pragma unroll
+      for (int sub = 0; sub < SB; ++sub) {
+        const unsigned char* st = v_ring + vs * RG::VB + sub * RG::VB1;
+        ScaleH sc[4];
         #pragma unroll
-        for (int w = 0; w < KU; ++w)
-          #pragma unroll
-          for (int n = 0; n < 2; ++n)
+        for (int w = 0; w < KU; ++w) {
+          if (w == 0 || RG::NVE > 1) {
+            const uint2 eb = *reinterpret_cast<const uint2*>(st + RG::VE + (g * KU + w) / 4 * RG::VES + 8 * t);
             #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              #pragma unroll
-              for (int k = 0; k < 4; ++k) O[w][n][nt][k] *= al[nt][k & 1];
-      }
-      // ---- O^T += V^T P^T.  Bytes at positions that no row sees may be anything:
-      // their scale becomes 0, which makes the values 0 and never NaN.
-      const int v_hi = min(len, any_hi);
-      const auto values = [&](auto W_) {
-        constexpr int w = decltype(W_)::value;
-        const unsigned word[4] = {tl.v[w].x, tl.v[w].y, tl.v[w].z, tl.v[w].w};
-        const uint2 eb = tl.ve[TL::NVE == 1 ? 0 : w];
-        #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          unsigned op[2][4];                                     // [pair of positions][dim]
-          #pragma unroll
-          for (int i2 = 0; i2 < 2; ++i2) {
-            const int i = 2 * j + i2;
-            unsigned by = prmt(eb.x, eb.y, (i | (8 + i) << 4 | (4 + i) << 8 | (12 + i) << 12));
-            if (!whole) {
-              const int p = base + 8 * t + i;
-              if (p >= v_hi || p < any_lo) by &= 0xFFFF0000u;
-              if (p + 4 >= v_hi || p + 4 < any_lo) by &= 0x0000FFFFu;
-            }
-            const ScaleH sc = scale_h(by);
-            const unsigned w8 = word[i] >> 8;
-            op[i2][0] = pair_h<0>(word[i], w8, sc);
-            op[i2][1] = pair_h<1>(word[i], w8, sc);
-            op[i2][2] = pair_h<2>(word[i], w8, sc);
-            op[i2][3] = pair_h<3>(word[i], w8, sc);
+            for (int i = 0; i < 4; ++i)                              // positions 8 t + i and 8 t + i + 4
+              sc[i] = scale_h(prmt(eb.x, eb.y, i * 0x0101 | 0x0080 | (4 + i) << 8 | (12 + i) << 12));
           }
+          const uint4 vv = *reinterpret_cast<const uint4*>(st + RG::v_place(t * (HD / 4) + g * KU + w) * 16);
+          const unsigned word[4] = {vv.x, vv.y, vv.z, vv.w};
           #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const unsigned fr[4] = {op[0][2 * n], op[0][2 * n + 1], op[1][2 * n], op[1][2 * n + 1]};
+          for (int j = 0; j < 2; ++j) {
+            unsigned op[2][4];                                     // [pair of positions][dim]
+            pairs_h(mg, word[2 * j], sc[2 * j], op[0]);
+            pairs_h(mg, word[2 * j + 1], sc[2 * j + 1], op[1]);
             #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int n = 0; n < 2; ++n) {
+              const unsigned fr[4] = {op[0][2 * n], op[0][2 * n + 1], op[1][2 * n], op[1][2 * n + 1]};
               #pragma unroll
-              for (int k = 0; k < PS; ++k) mma_f16(O[w][n][nt], fr, make_uint2(P[k][2 * j][nt], P[k][2 * j + 1][nt]));
+              for (int nt = 0; nt < NT; ++nt)
+                #pragma unroll
+                for (int k = 0; k < PS; ++k)
+                  mma_f16(O[w][n][nt], fr, make_uint2(P[k][sub * 4 + 2 * j][nt], P[k][sub * 4 + 2 * j + 1][nt]));
+            }
           }
         }
-      };
-      values(std::integral_constant<int, 0>{});
-      if constexpr (KU > 1) values(std::integral_constant<int, 1>{});
-      if constexpr (KU > 2) values(std::integral_constant<int, 2>{});
-      if constexpr (KU > 3) values(std::integral_constant<int, 3>{});
+      }
+    };
+    // Bytes at positions that no row sees may be anything; exponent 0 makes
+    // their values 0 (and never NaN, which a weight of 0 would not remove).
+    const int v_hi = min(len, any_hi);
+    const auto clear = [&](int vs, int base) {
+      #pragma unroll
+      for (int sub = 0; sub < SB; ++sub) {
+        const int p = base + 32 * sub + lane;
+        if (p >= v_hi || p < any_lo)
+          for (int tile = 0; tile < HD / 16; ++tile) v_ring[vs * RG::VB + sub * RG::VB1 + RG::VE + tile * RG::VES + lane] = 0;
+      }
+      __syncwarp();
     };
 
+    // The scores of a block are computed beside the accumulation of the one
+    // before: two independent chains for the scheduler.
     if (first + warp < last) {
-      int blk = first + warp;
-      TL cur, nxt;
-      load(cur, blk * BLK, page_at(blk * BLK + 4 * g), page_at(blk * BLK + 8 * t));
-      int pk = -1, pv = -1;
-      if (blk + W < last) { pk = page_at((blk + W) * BLK + 4 * g); pv = page_at((blk + W) * BLK + 8 * t); }
-      while (blk < last) {
-        const int next = blk + W;
-        if (next < last) {
-          load(nxt, next * BLK, pk, pv);
-          if (next + W < last) { pk = page_at((next + W) * BLK + 4 * g); pv = page_at((next + W) * BLK + 8 * t); }
+      int blk = first + warp, ahead = blk;
+      pages(blk * BLK);
+      const auto fetch = [&](int ks, int vs) {                        // the block `ahead`, and the next one's pages
+        __syncwarp();
+        if (ahead < last) {
+          load(ks, vs, ahead * BLK);
+          ahead += W;
+          if (ahead < last) pages(ahead * BLK);
         }
-        compute(cur, blk * BLK);
-        cur = nxt;
-        blk = next;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      #pragma unroll
+      for (int i = 0; i < STAGES; ++i) fetch(i, i);
+      int ks = 0, vs = 0;
+      const auto arrive = [&]() {                                     // block blk is here; is it whole?
+        asm volatile("cp.async.wait_group %0;" :: "n"(STAGES - 1) : "memory");
+        __syncwarp();
+        const int base = blk * BLK;
+        const bool whole = base + BLK <= all_hi && base >= all_lo;
+        if (!whole) clear(vs, base);
+        return whole;
+      };
+      bool whole = arrive();
+      scores(ks);
+      weights(blk * BLK, whole);
+      fetch(ks, STAGES);
+      for (;;) {
+        const int before = vs;
+        blk += W;
+        if (blk >= last) break;
+        ks = ks + 1 == STAGES ? 0 : ks + 1;
+        vs = vs == STAGES ? 0 : vs + 1;
+        whole = arrive();
+        scores(ks);
+        accumulate(before);
+        weights(blk * BLK, whole);
+        fetch(ks, before);
       }
+      accumulate(vs);
     }
+    __syncthreads();                                                  // the rings become the joining buffers
 
     // ---- join the warps
     #pragma unroll
@@ -582,7 +750,7 @@ __global__ void __launch_bounds__(W * 32) attn_kernel(const AttnArgs a) {
         #pragma unroll
         for (int o = 4; o < 32; o <<= 1) lsum[nt][c] += __shfl_xor_sync(0xffffffffu, lsum[nt][c], o);
         const int r = nt * 8 + 2 * t + c;
-        if (g == 0) { s_m[warp * NR + r] = m[nt][c]; s_l[warp * NR + r] = lsum[nt][c]; }
+        if (g == 0) { s_m[warp * NR + r] = m[nt][c] * a.scale_log2; s_l[warp * NR + r] = lsum[nt][c]; }
         #pragma unroll
         for (int w = 0; w < KU; ++w)
           #pragma unroll
@@ -592,6 +760,13 @@ __global__ void __launch_bounds__(W * 32) attn_kernel(const AttnArgs a) {
       }
     __syncthreads();
     const bool full = x == it.start && xe == it.end;
+    if (x == it.start && xe < it.end && tid == 0) {
+      // the parts end at the last boundary below the item's end, unless that was moved onto it
+      const long long c = blockIdx.x;
+      long long e = min(sch.geff, div_small(it.end * sch.geff + sch.total - 1, sch.total));
+      while (e - 1 > c + 1 && bound<NR, BLK>(a, sch, e - 1) >= it.end) --e;
+      a.cuts[c] = Cut{(int)(e - c), it.q.q0, rows, r0, h * a.group, {0, 0, 0}};
+    }
     float* part = a.part + ((long long)blockIdx.x * 2 + (x > it.start ? 0 : 1)) * NR * (HD + 2);
     for (int i = tid; i < rows * (HD / 4); i += W * 32) {
       const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
@@ -616,7 +791,7 @@ __global__ void __launch_bounds__(W * 32) attn_kernel(const AttnArgs a) {
         dst[1] = from_f<T>(o.y * inv);
         dst[2] = from_f<T>(o.z * inv);
         dst[3] = from_f<T>(o.w * inv);
-        if (d == 0 && a.lse) a.lse[(long long)(it.q.q0 + j) * a.HQ + head] = L == 0.f ? -INFINITY : (M + log2f(L) - P_EXP) * LN2;
+        if (d == 0 && a.lse) a.lse[(long long)(it.q.q0 + j) * a.HQ + head] = L == 0.f ? -INFINITY : (M + log2f(L) - P_EXP<PS>) * LN2;
       } else {
         *reinterpret_cast<float4*>(part + r * HD + d) = o;
         if (d == 0) { part[NR * HD + r] = M; part[NR * HD + NR + r] = L; }
@@ -631,38 +806,24 @@ __global__ void __launch_bounds__(W * 32) attn_kernel(const AttnArgs a) {
         it.start = it.end;
         it.end += it.q.nb;
       } else {
-        it = item_at<NR>(a, sch, x);
+        it = item_at<NR, BLK>(a, sch, x);
       }
     }
   }
 }
 
-// Joins the partial sums of the items that CTA boundary blockIdx.x cuts first.
+// Joins the partial sums of the item that CTA blockIdx.x began and others
+// ended, part after part in their order.
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(128) join_kernel(const AttnArgs a) {
-  constexpr int NR = NT * 8, Q = HD / 4, NG = 128 / Q;          // NG groups of threads share the parts
-  __shared__ Sched sch;
+__global__ void __launch_bounds__(256) join_kernel(const AttnArgs a) {
+  constexpr int NR = NT * 8, Q = HD / 4, NG = 256 / Q;          // NG groups of threads share the parts
   __shared__ float4 s_o[NG][Q];
   __shared__ float s_m[NG], s_l[NG];
-  make_sched<NR>(a, sch, 128);
-  const long long i = (long long)blockIdx.x + 1;
-  long long x = 0;
-  Item it;
-  bool mine = i < sch.geff && sch.total > 0;
-  if (mine) {
-    x = bound<NR>(a, sch, i);
-    mine = x < sch.total;
-    if (mine) {
-      it = item_at<NR>(a, sch, x);
-      mine = x > it.start && bound<NR>(a, sch, i - 1) <= it.start;
-    }
-  }
-  if (!mine) return;
-  long long i_end = i + 1;                                       // CTAs i - 1 .. i_end - 1 hold parts
-  while (i_end < sch.geff && bound<NR>(a, sch, i_end) < it.end) ++i_end;
-  const int n = (int)(i_end - i) + 1;
-  const int rt = it.q.rt, h = it.idx / rt, r0 = (it.idx - h * rt) * NR, rows = min(NR, it.q.n_q * a.group - r0);
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 c0 = __ldcg(reinterpret_cast<const int4*>(a.cuts + blockIdx.x));
+  const int n = c0.x, rows = c0.z;
+  if (n == 0) return;
+  const int head0 = __ldcg(&a.cuts[blockIdx.x].head0);
   const int grp = threadIdx.x / Q, d4 = threadIdx.x % Q;
   for (int r = blockIdx.y; r < rows; r += gridDim.y) {
     float M = -INFINITY, L = 0.f;
@@ -670,8 +831,7 @@ __global__ void __launch_bounds__(128) join_kernel(const AttnArgs a) {
     if (grp < NG) {
       #pragma unroll 4
       for (int k = grp; k < n; k += NG) {
-        const long long cta = i - 1 + k;
-        const float* part = a.part + (cta * 2 + (k ? 0 : 1)) * NR * (HD + 2);
+        const float* part = a.part + ((long long)(blockIdx.x + k) * 2 + (k ? 0 : 1)) * NR * (HD + 2);
         const float mk = __ldcg(part + NR * HD + r), lk = __ldcg(part + NR * HD + NR + r);
         const float4 v = __ldcg(reinterpret_cast<const float4*>(part + r * HD) + d4);
         const float mn = fmaxf(M, mk), ref = mn == -INFINITY ? 0.f : mn;
@@ -699,42 +859,42 @@ __global__ void __launch_bounds__(128) join_kernel(const AttnArgs a) {
         L += s_l[k] * f;
         o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
       }
-      const int R = r0 + r, j = R / a.group, head = h * a.group + R - j * a.group;
+      const int R = c0.w + r, j = R / a.group, head = head0 + R - j * a.group;
       const float inv = L == 0.f ? 0.f : V_UP / L;
-      T* dst = static_cast<T*>(a.out) + (long long)(it.q.q0 + j) * a.o_ts + (long long)head * a.o_hs + d4 * 4;
+      T* dst = static_cast<T*>(a.out) + (long long)(c0.y + j) * a.o_ts + (long long)head * a.o_hs + d4 * 4;
       dst[0] = from_f<T>(o.x * inv);
       dst[1] = from_f<T>(o.y * inv);
       dst[2] = from_f<T>(o.z * inv);
       dst[3] = from_f<T>(o.w * inv);
-      if (d4 == 0 && a.lse) a.lse[(long long)(it.q.q0 + j) * a.HQ + head] = L == 0.f ? -INFINITY : (mm + log2f(L) - P_EXP) * LN2;
+      if (d4 == 0 && a.lse) a.lse[(long long)(c0.y + j) * a.HQ + head] = L == 0.f ? -INFINITY : (mm + log2f(L) - P_EXP<Kind<T>::PS>) * LN2;
     }
     __syncthreads();
   }
 }
 
-template <int NT> constexpr int warps_of() { return NT == 4 ? 4 : 8; }
-
 template <typename T, int HD, int NT>
 cudaError_t launch_attn(AttnArgs a, int n_sm, float* ws, cudaStream_t s) {
-  constexpr int W = warps_of<NT>(), NR = NT * 8;
-  constexpr size_t smem = (size_t)(HD / 16) * NT * Kind<T>::QS * 32 * 8 + (size_t)W * NR * (HD + 2) * 4;
-  static_assert(smem <= 200 * 1024, "shared memory");
-  auto* kern = attn_kernel<T, HD, NT, W>;
+  using SH = Shape<HD, NT>;
+  constexpr int W = SH::W, NR = NT * 8;
+  constexpr size_t smem = SH::template smem<Kind<T>::QS>();
+  static_assert(smem + 2048 <= 227 * 1024, "shared memory");
+  auto* kern = attn_kernel<T, HD, NT>;
   cudaError_t e;
-  if (smem > 48 * 1024) {
+  if (smem > 40 * 1024) {                                          // static shared memory counts, too
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  a.grid = n_sm * (512 / (W * 32));
-  a.part = ws;
+  a.grid = n_sm * SH::CTAS;
+  a.cuts = reinterpret_cast<Cut*>(ws);
+  a.part = reinterpret_cast<float*>(a.cuts + a.grid);
   kern<<<a.grid, W * 32, smem, s>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   // items of at most MINB blocks are never cut
-  if ((long long)a.b.max_pages * a.b.page <= MINB * BLK) return cudaSuccess;
+  if ((long long)a.b.max_pages * a.b.page <= MINB * BLK_OF<HD>) return cudaSuccess;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.grid - 1, NR < 8 ? NR : 8);
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(a.grid, 4);
+  cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -753,7 +913,7 @@ int pick_nt(const Batch& b, int group) {
 size_t ws_bytes(int hd, int n_sm) {
   size_t most = 0;
   for (int nt = 1; nt <= 4; nt *= 2) {
-    const size_t grid = (size_t)n_sm * (512 / ((nt == 4 ? 4 : 8) * 32)), b = grid * 2 * nt * 8 * (hd + 2) * 4;
+    const size_t grid = (size_t)n_sm * 4, b = grid * (sizeof(Cut) + 2 * nt * 8 * (hd + 2) * 4);
     most = b > most ? b : most;
   }
   return most;
@@ -817,7 +977,12 @@ extern "C" int bfp200_kv4_attention_dev(const bfp200_kv4_attention_args* in, voi
   a.group = a.HQ / a.b.H;
   a.causal = r.causal != 0;
   a.window = r.window;
-  a.scale_log2 = (float)(r.scale * 1.4426950408889634 * (r.dtype == BFP200_F16 ? 16.0 : 1.0));   // K is held times 2^-4 there
+  const double sl = std::fabs(r.scale) * 1.4426950408889634 * (r.dtype == BFP200_F16 ? 16.0 : 1.0);   // K is held times 2^-4 there
+  if (sl > 1e30) return bad("scale is too large");
+  a.scale_log2 = (float)std::fmax(sl, 1e-30);
+  a.slack[0] = SLACK<1> / a.scale_log2;
+  a.slack[1] = SLACK<2> / a.scale_log2;
+  a.q_flip = r.scale < 0 ? 0x80008000u : 0u;
   a.grid = 0;
   a.part = nullptr;
   const int nt = pick_nt(a.b, a.group), hd = (int)r.batch.HD;
