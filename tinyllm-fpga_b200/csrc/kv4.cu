@@ -9,6 +9,7 @@
 // inverse (the gradient) negates s.  All three kernels are bound by memory.
 #include "kv4.cuh"
 
+#include <cstring>
 #include <exception>
 #include <mutex>
 #include <string>
@@ -74,6 +75,11 @@ int cuda_fail(const char* who, cudaError_t e) {
   return bfp200_set_error(BFP200_ECUDA, std::string(who) + ": " + cudaGetErrorString(e));
 }
 
+__device__ __forceinline__ unsigned u_of(__half2 h) { return *reinterpret_cast<unsigned*>(&h); }
+__device__ __forceinline__ unsigned u_of(__nv_bfloat162 h) { return *reinterpret_cast<unsigned*>(&h); }
+__device__ __forceinline__ __half2 h2_of(unsigned u) { return *reinterpret_cast<__half2*>(&u); }
+__device__ __forceinline__ __nv_bfloat162 b2_of(unsigned u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
+
 struct Rot {
   const float* table;     // [n_pos][rot / 2][2] (cos, sin)
   const int* positions;   // [T], or null: the token's cache position
@@ -104,7 +110,7 @@ struct RopeArgs {
   float sign;
 };
 
-template <typename T, int VE, bool INTER, bool ALIGNED>
+template <typename T, int VE, bool INTER, bool ALIGNED, bool NC>
 __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
   const long long id = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   const int per = a.tasks * a.hsplit;
@@ -133,14 +139,14 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
     for (int h = h0; h < h1; ++h) {
       if constexpr (INTER) {
         float v[W];
-        load_vec<T, W, ALIGNED>(x + h * a.x_hs + d, v);
+        load_vec<T, W, ALIGNED, NC>(x + h * a.x_hs + d, v);
         #pragma unroll
         for (int i = 0; i < NP; ++i) turn(v[2 * i], v[2 * i + 1], c[i], s[i]);
         store_vec<T, W, ALIGNED>(o + h * a.o_hs + d, v);
       } else {
         float v[W], w[W];
-        load_vec<T, W, ALIGNED>(x + h * a.x_hs + d, v);
-        load_vec<T, W, ALIGNED>(x + h * a.x_hs + d + a.rot / 2, w);
+        load_vec<T, W, ALIGNED, NC>(x + h * a.x_hs + d, v);
+        load_vec<T, W, ALIGNED, NC>(x + h * a.x_hs + d + a.rot / 2, w);
         #pragma unroll
         for (int i = 0; i < NP; ++i) turn(v[i], w[i], c[i], s[i]);
         store_vec<T, W, ALIGNED>(o + h * a.o_hs + d, v);
@@ -153,7 +159,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
     for (int h = h0; h < h1; ++h) {
       if constexpr (ALIGNED) {
         float v[W];
-        load_vec<T, W, true>(x + h * a.x_hs + d, v);
+        load_vec<T, W, true, NC>(x + h * a.x_hs + d, v);
         store_vec<T, W, true>(o + h * a.o_hs + d, v);
       } else {
         #pragma unroll
@@ -181,16 +187,19 @@ cudaError_t launch_rope(RopeArgs a, bool inter, cudaStream_t s) {
   const long long threads = (long long)a.T * a.tasks * a.hsplit, blocks = (threads + 255) / 256;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   const dim3 g((unsigned)blocks);
-  if (aligned && inter) rope_kernel<T, VE, true, true><<<g, 256, 0, s>>>(a);
-  else if (aligned) rope_kernel<T, VE, false, true><<<g, 256, 0, s>>>(a);
-  else if (inter) rope_kernel<T, 1, true, false><<<g, 256, 0, s>>>(a);
-  else rope_kernel<T, 1, false, false><<<g, 256, 0, s>>>(a);
+  const bool apart = a.x != a.out;              // not in place: the read-only path (16383 x 40 x 128 floats: 122 us, else 133)
+  if (aligned && inter) (apart ? rope_kernel<T, VE, true, true, true> : rope_kernel<T, VE, true, true, false>)<<<g, 256, 0, s>>>(a);
+  else if (aligned) (apart ? rope_kernel<T, VE, false, true, true> : rope_kernel<T, VE, false, true, false>)<<<g, 256, 0, s>>>(a);
+  else if (inter) rope_kernel<T, 1, true, false, false><<<g, 256, 0, s>>>(a);
+  else rope_kernel<T, 1, false, false, false><<<g, 256, 0, s>>>(a);
   return cudaGetLastError();
 }
 
 // ---------------------------------------------------------------------------
-// append: rows of a token (keys, values, then queries) are taken by groups of
-// LPR lanes, 8 dims a lane; two lanes hold a tile.
+// append: a warp takes rows of one token (keys, values, then queries), LPR
+// lanes a row, 8 dims a lane; two lanes hold a tile.  The token's table entries
+// stay in registers over the rows, and the rows' loads are issued before the
+// token's place is looked up.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   Batch b;
@@ -198,200 +207,331 @@ struct AppendArgs {
   const void *k, *v, *q;
   void* q_out;
   long long k_ts, k_hs, v_ts, v_hs, q_ts, q_hs, o_ts, o_hs;
-  int HQ, rows, row_groups;
+  int HQ, passes, groups, group_passes;     // groups of passes of a token, one a warp
+  int table_vec;                            // table rows can be read 16 bytes at a time
 };
 
 template <int HD> constexpr int LANES_PER_ROW = HD <= 32 ? 4 : HD <= 64 ? 8 : 16;
 
-// Rotates the 8 dims that this lane holds of a row.  Lanes of the row sit next
-// to each other; `exch` (HD floats of the row) is used where a pair's other
-// half is not a whole lane away.
-template <int HD>
-__device__ __forceinline__ void rotate8(float (&f)[8], int li, const float* row, int rot, bool inter, float* exch) {
-  const int d0 = li * 8;
-  if (inter) {
+// 8 elements as they lie in memory.
+template <typename T> struct Raw8 { unsigned w[2 * sizeof(T)]; };
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ Raw8<T> load_raw(const T* p) {
+  Raw8<T> r;
+  if constexpr (ALIGNED) {
     #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (d0 + 2 * i < rot) {
-        const float2 cs = __ldg(reinterpret_cast<const float2*>(row) + d0 / 2 + i);
-        turn(f[2 * i], f[2 * i + 1], cs.x, cs.y);
-      }
-    return;
-  }
-  const int half = rot >> 1;
-  float o[8];                                            // the other elements of the pairs
-  if ((half & 7) == 0) {
-    const int up = half >> 3;
-    const int lane = threadIdx.x & 31;
-    const bool in = d0 < rot;
-    const int src = !in ? lane : d0 < half ? lane + up : lane - up;
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, f[i], src);
-    if (in) {
-      const bool first = d0 < half;
-      const float2* cs2 = reinterpret_cast<const float2*>(row) + (first ? d0 : d0 - half);
-      #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 cs = __ldg(cs2 + i);
-        float a = first ? f[i] : o[i], b = first ? o[i] : f[i];
-        turn(a, b, cs.x, cs.y);
-        f[i] = first ? a : b;
-      }
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+      r.w[4 * i] = v.x; r.w[4 * i + 1] = v.y; r.w[4 * i + 2] = v.z; r.w[4 * i + 3] = v.w;
     }
+  } else if constexpr (sizeof(T) == 4) {
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) r.w[i] = __ldcs(reinterpret_cast<const unsigned*>(p) + i);
+  } else {
+    const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = __ldcs(h + 2 * i) | (unsigned)__ldcs(h + 2 * i + 1) << 16;
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void to_floats(const Raw8<T>& r, float (&f)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r.w[i]);
   } else {
     #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (d0 + i < HD) exch[d0 + i] = f[i];
-    __syncwarp();
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int d = d0 + i;
-      if (d < rot) {
-        const bool first = d < half;
-        const int j = first ? d : d - half;
-        const float2 cs = __ldg(reinterpret_cast<const float2*>(row) + j);
-        float a = exch[j], b = exch[j + half];
-        turn(a, b, cs.x, cs.y);
-        f[i] = first ? a : b;
-      }
+    for (int i = 0; i < 4; ++i) {
+      T e[2];
+      memcpy(e, &r.w[i], 4);
+      f[2 * i] = to_f(e[0]);
+      f[2 * i + 1] = to_f(e[1]);
     }
-    __syncwarp();
   }
 }
 
+// The sequence of token t (see find_seq); in a step of one token each it is t.
+__device__ __forceinline__ int seq_of_token(const Batch& b, int t) {
+  if (b.T == b.n_seq && __ldg(b.q_start + t) == t && __ldg(b.q_start + t + 1) == t + 1) return t;
+  return find_seq(b.q_start, b.n_seq, t);
+}
+
 template <typename T, int HD, bool ALIGNED>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
-  constexpr int LPR = LANES_PER_ROW<HD>, RPW = 32 / LPR, REC9 = HD * 9 / 8;
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) append_kernel(const AppendArgs a) {
+  constexpr int LPR = LANES_PER_ROW<HD>, RPW = 32 / LPR, REC9 = HD * 9 / 8, UNR = 4;
   __shared__ float s_exch[8][RPW][HD];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int li = lane % LPR, ri = lane / LPR;
+  const int li = lane % LPR, ri = lane / LPR, d0 = li * 8;
   const long long wid = (long long)blockIdx.x * 8 + warp;
-  const int t = (int)(wid / a.row_groups), rg = (int)(wid % a.row_groups);
+  const int t = (int)(wid / a.groups), grp = (int)(wid - (long long)t * a.groups);
   if (t >= a.b.T) return;
-  const int seq = find_seq(a.b.q_start, a.b.n_seq, t);
+  // A pass is RPW rows of one kind: PH passes of keys, PH of values, then queries.
+  const int H = a.b.H, PH = (H + RPW - 1) / RPW, p_end = min(a.passes, (grp + 1) * a.group_passes);
+  const T* const kb = static_cast<const T*>(a.k) + t * a.k_ts + d0;
+  const T* const vb = static_cast<const T*>(a.v) + t * a.v_ts + d0;
+  const T* const qb = static_cast<const T*>(a.q) + t * a.q_ts + d0;
+  T* const ob = static_cast<T*>(a.q_out) + t * a.o_ts + d0;
+  Raw8<T> raw[UNR];
+  const auto load = [&](int p0) {
+    #pragma unroll
+    for (int k = 0; k < UNR; ++k) {
+      const int p = p0 + k;
+      if (p >= p_end) break;
+      const int h = (p < PH ? p : p < 2 * PH ? p - PH : p - 2 * PH) * RPW + ri;
+      raw[k] = Raw8<T>{};
+      if (d0 < HD && h < (p < 2 * PH ? H : a.HQ))
+        raw[k] = load_raw<T, ALIGNED>(p < PH ? kb + h * a.k_hs : p < 2 * PH ? vb + h * a.v_hs : qb + h * a.q_hs);
+    }
+  };
+  load(grp * a.group_passes);
+  const int seq = seq_of_token(a.b, t);
   const int q_end = __ldg(a.b.q_start + seq + 1);
   const int pos = __ldg(a.b.lens + seq) - q_end + t;
   const bool held = t >= __ldg(a.b.q_start + seq) && t < q_end && pos >= 0 && (pos >> a.b.page_shift) < a.b.max_pages;
   const int pg = held ? __ldg(a.b.bt + (long long)seq * a.b.bt_ld + (pos >> a.b.page_shift)) : -1;
   const bool store = held && (unsigned)pg < (unsigned)a.b.n_pages;
-  const float* row = nullptr;
-  if (a.r.table) {
+  const int rot = a.r.table ? a.r.rot : 0, half = rot >> 1;
+  // The lane's (cos, sin): of its 4 pairs (interleaved), or one for each of its
+  // dims, the sign of sin turned where the dim is the first of its pair.
+  const bool lanewise = (half & 7) == 0;                    // the pair's other dims are a whole lane's
+  float c[8], sn[8];
+  if (rot) {
     const int p = a.r.positions ? __ldg(a.r.positions + t) : pos;
-    row = a.r.table + (long long)min(max(p, 0), a.r.n_pos - 1) * a.r.rot;
-  }
-  const int slot = pos & (a.b.page - 1), page = a.b.page, H = a.b.H;
-  #pragma unroll 1
-  for (int k = 0; k < 4; ++k) {
-    const int rw = (rg * 4 + k) * RPW + ri;                       // row of this token
-    if ((rg * 4 + k) * RPW >= a.rows) break;
-    const bool on = rw < a.rows && li * 8 < HD;
-    const int what = rw < H ? 0 : rw < 2 * H ? 1 : 2;             // key, value, query
-    const int h = rw - what * H;
-    float f[8];
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = 0.f;
-    if (on) {
-      const T* p = what == 0 ? static_cast<const T*>(a.k) + t * a.k_ts + h * a.k_hs
-                 : what == 1 ? static_cast<const T*>(a.v) + t * a.v_ts + h * a.v_hs
-                             : static_cast<const T*>(a.q) + t * a.q_ts + h * a.q_hs;
-      load_vec<T, 8, ALIGNED>(p + li * 8, f);
-    }
-    if (row) {
-      float keep[8];
+    const float* row = a.r.table + (long long)min(max(p, 0), a.r.n_pos - 1) * rot;
+    if (a.r.inter) {
       #pragma unroll
-      for (int i = 0; i < 8; ++i) keep[i] = f[i];
-      rotate8<HD>(f, li, row, a.r.rot, a.r.inter, s_exch[warp][ri]);
-      if (what == 1) {
-        #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = keep[i];
+      for (int i = 0; i < 4; ++i) {
+        const float2 cs = d0 + 2 * i < rot ? __ldg(reinterpret_cast<const float2*>(row) + d0 / 2 + i) : make_float2(1.f, 0.f);
+        c[i] = cs.x;
+        sn[i] = cs.y;
+      }
+    } else if (lanewise && a.table_vec && d0 < rot) {
+      const float4* cs4 = reinterpret_cast<const float4*>(row + (d0 < half ? d0 : d0 - half) * 2);
+      const float sign = d0 < half ? -1.f : 1.f;
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 v = __ldg(cs4 + i);
+        c[2 * i] = v.x; c[2 * i + 1] = v.z;
+        sn[2 * i] = v.y * sign; sn[2 * i + 1] = v.w * sign;
+      }
+    } else {
+      #pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int d = d0 + i;
+        const float2 cs = d < rot ? __ldg(reinterpret_cast<const float2*>(row) + (d < half ? d : d - half)) : make_float2(1.f, 0.f);
+        c[i] = cs.x;
+        sn[i] = d < half ? -cs.y : cs.y;
       }
     }
+  }
+  const int src = !lanewise || d0 >= rot ? lane : d0 < half ? lane + (half >> 3) : lane - (half >> 3);
+  // a row turned, as floats
+  const auto rotate = [&](const Raw8<T>& r, float (&f)[8]) {
+    to_floats(r, f);
+    if (!rot) return;
+    if (a.r.inter) {
+      #pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (d0 + 2 * i < rot) turn(f[2 * i], f[2 * i + 1], c[i], sn[i]);
+    } else if (lanewise) {
+      Raw8<T> other;
+      #pragma unroll
+      for (int i = 0; i < (int)(2 * sizeof(T)); ++i) other.w[i] = __shfl_sync(0xffffffffu, r.w[i], src);
+      float o[8];                                           // the other elements of the pairs
+      to_floats(other, o);
+      if (d0 < rot) {
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(__fmul_rn(f[i], c[i]), __fmul_rn(o[i], sn[i]));   // a c - b s, or b c + a s
+      }
+    } else {
+      float* exch = s_exch[warp][ri];
+      #pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (d0 + i < HD) exch[d0 + i] = f[i];
+      __syncwarp();
+      #pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int d = d0 + i;
+        if (d < rot) f[i] = __fadd_rn(__fmul_rn(f[i], c[i]), __fmul_rn(exch[d < half ? d + half : d - half], sn[i]));
+      }
+      __syncwarp();
+    }
+  };
+  // the row's 8 nibbles of this lane, and their tile's exponent byte
+  const auto quantize = [&](const float (&f)[8], int& e) {
     float top = 0.f;
     #pragma unroll
     for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(f[i]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    if (!on) continue;
-    if (what == 2) {
-      store_vec<T, 8, ALIGNED>(static_cast<T*>(a.q_out) + t * a.o_ts + h * a.o_hs + li * 8, f);
-      continue;
-    }
-    if (!store) continue;
-    const int e = tile_e(top);
+    e = tile_e(top);
     const float up = pow2f(3 - e);
-    unsigned w = 0;
+    int w = 0;                                              // sum of m_i 16^i; adding 8 to every nibble makes them 0..15
     #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= nibble(f[i], up) << (4 * i);
-    uint8_t* rec = a.b.pool + ((long long)pg * H + h) * (page * REC9);
-    if (what == 0) {
-      *reinterpret_cast<unsigned*>(rec + ((slot >> 2) * (HD / 8) + li) * 16 + (slot & 3) * 4) = w;
-    } else {
-      uint8_t* vp = rec + page * HD / 2 + ((slot >> 3) * (HD / 4) + 2 * li) * 16 + (slot & 3) * 4 + (slot >> 2 & 1) * 2;
-      *reinterpret_cast<uint16_t*>(vp) = (uint16_t)w;
-      *reinterpret_cast<uint16_t*>(vp + 16) = (uint16_t)(w >> 16);
+    for (int i = 7; i >= 0; --i) w = w * 16 + mantissa(f[i], up);
+    return (unsigned)w + 0x88888888u;
+  };
+  const int slot = pos & (a.b.page - 1), page = a.b.page;
+  uint8_t* const rec0 = a.b.pool + (store ? (long long)pg * H : 0) * (page * REC9);
+  uint8_t* const k_at = rec0 + ((slot >> 2) * (HD / 8) + li) * 16 + (slot & 3) * 4;
+  uint8_t* const v_at = rec0 + page * HD / 2 + ((slot >> 3) * (HD / 4) + 2 * li) * 16 + (slot & 3) * 4 + (slot >> 2 & 1) * 2;
+  uint8_t* const e_at = rec0 + page * HD + li / 2 * page + slot;
+  #pragma unroll 1
+  for (int p0 = grp * a.group_passes; p0 < p_end; p0 += UNR) {
+    if (p0 != grp * a.group_passes) load(p0);
+    #pragma unroll
+    for (int k = 0; k < UNR; ++k) {
+      const int p = p0 + k;
+      if (p >= p_end) break;
+      float f[8];
+      if (p >= 2 * PH) {                                    // queries
+        const int h = (p - 2 * PH) * RPW + ri;
+        rotate(raw[k], f);
+        if (d0 < HD && h < a.HQ) store_vec<T, 8, ALIGNED>(ob + h * a.o_hs, f);
+      } else {
+        const bool key = p < PH;
+        const int h = (key ? p : p - PH) * RPW + ri;
+        if (key) rotate(raw[k], f);
+        else to_floats(raw[k], f);
+        int e;
+        const unsigned w = quantize(f, e);
+        if (!store || d0 >= HD || h >= H) continue;
+        const int off = h * (page * REC9);
+        if (key) {
+          *reinterpret_cast<unsigned*>(k_at + off) = w;
+        } else {
+          *reinterpret_cast<uint16_t*>(v_at + off) = (uint16_t)w;
+          *reinterpret_cast<uint16_t*>(v_at + off + 16) = (uint16_t)(w >> 16);
+        }
+        if ((li & 1) == 0) e_at[off + (key ? 0 : HD / 16 * page)] = (uint8_t)(e + 18);
+      }
     }
-    if ((li & 1) == 0) rec[page * HD + ((what * HD / 16) + li / 2) * page + slot] = (uint8_t)(e + 18);
   }
 }
 
 // ---------------------------------------------------------------------------
-// read: 8 consecutive tokens of one head per warp, keys then values; a lane
-// takes 8 dims of a token, so that the 8 tokens' bytes of one unit, which lie
-// next to each other, are read together.
+// read: a warp decodes octs of 8 positions, HD / 4 lanes a head: a key unit (4
+// positions x 8 dims) and a value unit (8 positions x 4 dims) a lane, 16 bytes
+// each.  An oct belongs to the warp that holds its first token.
 // ---------------------------------------------------------------------------
 struct ReadArgs {
   Batch b;
   void *k, *v;          // [T][H][HD]
+  int span;             // tokens of a warp
 };
+
+// 8 nibbles of a word times the 16-bit scales of its halves (2^(B - 21)), as the
+// pairs (n, n + 4); exact in both types.
+template <typename T>
+__device__ __forceinline__ void nibble_pairs(unsigned w, unsigned bytes, unsigned (&o)[4]) {
+  if constexpr (std::is_same<T, __half>::value) {
+    // 2^(B - 15) 2^-6 (the mask keeps a byte that stands for no position out of the other half)
+    const __half2 h = __hmul2(h2_of(bytes << 10 & 0x7C007C00u), __floats2half2_rn(0x1p-6f, 0x1p-6f));
+    #pragma unroll
+    for (int n = 0; n < 4; ++n)
+      o[n] = u_of(__hmul2(__hsub2(h2_of((w >> (4 * n) & 0x000F000Fu) | 0x64006400u), __floats2half2_rn(1032.f, 1032.f)), h));
+  } else {
+    const unsigned s = bytes * 128u + 0x35003500u;
+    const __nv_bfloat162 sc = b2_of(s), c = __hmul2(sc, __floats2bfloat162_rn(-136.f, -136.f));
+    #pragma unroll
+    for (int n = 0; n < 4; ++n) o[n] = u_of(__hfma2(b2_of((w >> (4 * n) & 0x000F000Fu) | 0x43004300u), sc, c));
+  }
+}
+// N pairs of 16-bit values to T (bfloat16 pairs widen to float by a shift).
+template <typename T, int N>
+__device__ __forceinline__ void put(T* p, const unsigned (&v)[N]) {
+  if constexpr (std::is_same<T, float>::value) {
+    #pragma unroll
+    for (int i = 0; i < N; i += 2)
+      *reinterpret_cast<uint4*>(p + 2 * i) = make_uint4(v[i] << 16, v[i] & 0xFFFF0000u, v[i + 1] << 16, v[i + 1] & 0xFFFF0000u);
+  } else if constexpr (N == 4) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
+  } else {
+    *reinterpret_cast<uint2*>(p) = make_uint2(v[0], v[1]);
+  }
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
-  constexpr int REC9 = HD * 9 / 8;
+  constexpr int REC9 = HD * 9 / 8, LH = HD / 4, HPW = 32 / LH;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int H = a.b.H, page = a.b.page, hg = (H + HPW - 1) / HPW;
   const long long wid = (long long)blockIdx.x * 8 + warp;
-  const int H = a.b.H, page = a.b.page;
-  const long long t0 = wid / H * 8;
-  const int h = (int)(wid % H);
+  const long long t0 = wid / hg * a.span;
+  const int sub = lane / LH, u = lane % LH, h = (int)(wid % hg) * HPW + sub;
   if (t0 >= a.b.T) return;
+  const int t_end = (int)min((long long)a.b.T, t0 + a.span);
+  const bool on = sub < HPW && h < H;
   int seq = find_seq(a.b.q_start, a.b.n_seq, (int)t0);
-  const long long t = t0 + (lane & 7);
-  if (t >= a.b.T) return;
-  while (seq + 1 < a.b.n_seq && __ldg(a.b.q_start + seq + 1) <= t) ++seq;
-  const int q_end = __ldg(a.b.q_start + seq + 1);
-  const int pos = __ldg(a.b.lens + seq) - q_end + (int)t;
-  const bool held = t >= __ldg(a.b.q_start + seq) && t < q_end && pos >= 0 && (pos >> a.b.page_shift) < a.b.max_pages;
-  const long long at = held ? record_of(a.b, seq, pos, h, page * REC9) : -1;
-  const int slot = pos & (page - 1);
-  const uint8_t* rec = a.b.pool + (at < 0 ? 0 : at);
-  #pragma unroll
-  for (int u = 0; u < HD / 8; u += 4) {
-    const int un = u + (lane >> 3);                            // 8 dims
-    unsigned kw = 0x88888888u, vw = 0x88888888u, ke = 21, ve = 21;
-    if (at >= 0) {
-      kw = __ldg(reinterpret_cast<const unsigned*>(rec + ((slot >> 2) * (HD / 8) + un) * 16 + (slot & 3) * 4));
-      const uint8_t* vp = rec + page * HD / 2 + ((slot >> 3) * (HD / 4) + 2 * un) * 16 + (slot & 3) * 4 + (slot >> 2 & 1) * 2;
-      vw = __ldg(reinterpret_cast<const unsigned short*>(vp)) |
-           ((unsigned)__ldg(reinterpret_cast<const unsigned short*>(vp + 16)) << 16);
-      ke = __ldg(rec + page * HD + (un >> 1) * page + slot);
-      ve = __ldg(rec + page * HD + (HD / 16 + (un >> 1)) * page + slot);
+  int t = (int)t0;
+  while (t < t_end) {                                       // the same for every lane
+    while (seq + 1 < a.b.n_seq && __ldg(a.b.q_start + seq + 1) <= t) ++seq;
+    const int q0 = __ldg(a.b.q_start + seq), q1 = __ldg(a.b.q_start + seq + 1);
+    const int pos = __ldg(a.b.lens + seq) - q1 + t;
+    const bool mine = t >= q0 && t < q1 && pos >= 0 && (pos >> a.b.page_shift) < a.b.max_pages;
+    if (!mine) {                                            // a token without a place reads as zeros
+      const unsigned z[4] = {0, 0, 0, 0};
+      if (on && u < HD / 8) {
+        put<T, 4>(static_cast<T*>(a.k) + ((long long)t * H + h) * HD + u * 8, z);
+        put<T, 4>(static_cast<T*>(a.v) + ((long long)t * H + h) * HD + u * 8, z);
+      }
+      ++t;
+      continue;
     }
-    const float ks = pow2f((int)ke - 21), vs = pow2f((int)ve - 21);
-    float kf[8], vf[8];
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      kf[i] = (float)((int)(kw >> (4 * i) & 15u) - 8) * ks;
-      vf[i] = (float)((int)(vw >> (4 * i) & 15u) - 8) * vs;
+    if (t > q0 && (pos & 7)) { ++t; continue; }             // inside an oct of another warp's, or of the last round
+    const int o = pos & 7, n = min(min(8 - o, q1 - t), a.b.T - t);   // tokens t .. t + n - 1 at places o .. o + n - 1 of the oct
+    const int pg = __ldg(a.b.bt + (long long)seq * a.b.bt_ld + (pos >> a.b.page_shift));
+    const bool there = (unsigned)pg < (unsigned)a.b.n_pages;
+    const int slot = pos & (page - 8);
+    if (on) {
+      const uint8_t* rec = a.b.pool + (there ? ((long long)pg * H + h) * (page * REC9) : 0);
+      uint4 kw, vw;
+      unsigned ke;
+      uint2 ve;
+      const int quad = u / (HD / 8), ku = u % (HD / 8);
+      if (there) {
+        kw = __ldg(reinterpret_cast<const uint4*>(rec + ((slot >> 2) * (HD / 8) + u) * 16));
+        vw = __ldg(reinterpret_cast<const uint4*>(rec + page * HD / 2 + ((slot >> 3) * (HD / 4) + u) * 16));
+        ke = __ldg(reinterpret_cast<const unsigned*>(rec + page * HD + (ku >> 1) * page + slot + 4 * quad));
+        ve = __ldg(reinterpret_cast<const uint2*>(rec + page * HD + (HD / 16 + (u >> 2)) * page + slot));
+      } else {
+        kw = vw = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+        ke = 0x15151515u;
+        ve = make_uint2(0x15151515u, 0x15151515u);
+      }
+      const unsigned kword[4] = {kw.x, kw.y, kw.z, kw.w}, vword[4] = {vw.x, vw.y, vw.z, vw.w};
+      T* kp = static_cast<T*>(a.k) + ((long long)(t - o) * H + h) * HD + ku * 8;
+      T* vp = static_cast<T*>(a.v) + ((long long)(t - o) * H + h) * HD + u * 4;
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        unsigned op[4];
+        const unsigned kb = (ke >> (8 * i) & 0xFFu) * 0x10001u;
+        nibble_pairs<T>(kword[i], kb, op);
+        const unsigned row[4] = {__byte_perm(op[0], op[1], 0x5410), __byte_perm(op[2], op[3], 0x5410),
+                                 __byte_perm(op[0], op[1], 0x7632), __byte_perm(op[2], op[3], 0x7632)};
+        const int pk = 4 * quad + i;
+        if (pk >= o && pk < o + n) put<T, 4>(kp + (long long)pk * H * HD, row);
+        nibble_pairs<T>(vword[i], (ve.x >> (8 * i) & 0xFFu) | (ve.y >> (8 * i) & 0xFFu) << 16, op);
+        const unsigned lo[2] = {__byte_perm(op[0], op[1], 0x5410), __byte_perm(op[2], op[3], 0x5410)};
+        const unsigned hi[2] = {__byte_perm(op[0], op[1], 0x7632), __byte_perm(op[2], op[3], 0x7632)};
+        if (i >= o && i < o + n) put<T, 2>(vp + (long long)i * H * HD, lo);
+        if (i + 4 >= o && i + 4 < o + n) put<T, 2>(vp + (long long)(i + 4) * H * HD, hi);
+      }
     }
-    const long long o = (t * H + h) * HD + un * 8;
-    store_vec<T, 8, true>(static_cast<T*>(a.k) + o, kf);
-    store_vec<T, 8, true>(static_cast<T*>(a.v) + o, vf);
+    t += n;
   }
 }
 
 template <typename T, int HD>
 cudaError_t launch_append(AppendArgs a, bool aligned, cudaStream_t s) {
   constexpr int RPW = 32 / LANES_PER_ROW<HD>;
-  a.row_groups = (a.rows + 4 * RPW - 1) / (4 * RPW);
-  const long long blocks = ((long long)a.b.T * a.row_groups + 7) / 8;
+  a.passes = 2 * ((a.b.H + RPW - 1) / RPW) + (a.HQ + RPW - 1) / RPW;
+  // All rows of a token by one warp, or batches of 4 passes by several while the GPU has room.
+  int batches = (a.passes + 3) / 4, each = batches;
+  while (each > 1 && (long long)a.b.T * ((batches + each - 1) / each) < 148LL * 32) each = (each + 1) / 2;
+  a.group_passes = each * 4;
+  a.groups = (batches + each - 1) / each;
+  a.table_vec = a.r.table && a.r.rot % 4 == 0 && reinterpret_cast<uintptr_t>(a.r.table) % 16 == 0;
+  const long long blocks = ((long long)a.b.T * a.groups + 7) / 8;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   if (aligned) append_kernel<T, HD, true><<<(unsigned)blocks, 256, 0, s>>>(a);
   else append_kernel<T, HD, false><<<(unsigned)blocks, 256, 0, s>>>(a);
@@ -399,8 +539,13 @@ cudaError_t launch_append(AppendArgs a, bool aligned, cudaStream_t s) {
 }
 
 template <typename T, int HD>
-cudaError_t launch_read(const ReadArgs& a, cudaStream_t s) {
-  const long long blocks = (((long long)a.b.T + 7) / 8 * a.b.H + 7) / 8;
+cudaError_t launch_read(ReadArgs a, cudaStream_t s) {
+  constexpr int HPW = 32 / (HD / 4);
+  const long long hg = (a.b.H + HPW - 1) / HPW;
+  // 8 tokens a warp are one oct of a prompt, but 8 octs of a step's sequences:
+  // one after the other only where the GPU is full without.
+  a.span = a.b.T * hg <= 148LL * 64 ? 1 : 8;
+  const long long blocks = (((long long)a.b.T + a.span - 1) / a.span * hg + 7) / 8;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   read_kernel<T, HD><<<(unsigned)blocks, 256, 0, s>>>(a);
   return cudaGetLastError();
@@ -485,8 +630,7 @@ extern "C" int bfp200_kv4_append_dev(const bfp200_kv4_append_args* in, void* str
   a.k_ts = r.k_ts; a.k_hs = r.k_hs; a.v_ts = r.v_ts; a.v_hs = r.v_hs;
   a.q_ts = r.q_ts; a.q_hs = r.q_hs; a.o_ts = r.o_ts; a.o_hs = r.o_hs;
   a.HQ = (int)r.H_Q;
-  a.rows = 2 * a.b.H + a.HQ;
-  a.row_groups = 0;
+  a.passes = a.groups = a.group_passes = a.table_vec = 0;
   long long strides = r.k_ts | r.k_hs | r.v_ts | r.v_hs;
   if (r.H_Q) strides |= r.q_ts | r.q_hs | r.o_ts | r.o_hs;
   const bool aligned = all % 16 == 0 && strides * es % 16 == 0;
@@ -516,6 +660,7 @@ extern "C" int bfp200_kv4_read_dev(const bfp200_kv4_read_args* in, void* stream)
   int n_sm = 0;
   if (int rc = device_ready(who, &n_sm)) return rc;
   a.k = in->k_out_dev; a.v = in->v_out_dev;
+  a.span = 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = by_hd((int)in->batch.HD, [&](auto hd) {
     constexpr int N = decltype(hd)::value;

@@ -52,14 +52,15 @@ template <> __device__ __forceinline__ float from_f<float>(float x) { return x; 
 template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// VE consecutive elements, as 16-byte words when ALIGNED.
-template <typename T, int VE, bool ALIGNED>
+// VE consecutive elements, as 16-byte words when ALIGNED; by the read-only path
+// (NC) where nothing is written in place.
+template <typename T, int VE, bool ALIGNED, bool NC>
 __device__ __forceinline__ void load_vec(const T* p, float (&f)[VE]) {
   if constexpr (ALIGNED) {
     constexpr int NW = VE * (int)sizeof(T) / 16;
     alignas(16) T v[VE];
     #pragma unroll
-    for (int i = 0; i < NW; ++i) reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    for (int i = 0; i < NW; ++i) reinterpret_cast<uint4*>(v)[i] = NC ? __ldg(reinterpret_cast<const uint4*>(p) + i) : reinterpret_cast<const uint4*>(p)[i];
     #pragma unroll
     for (int i = 0; i < VE; ++i) f[i] = to_f(v[i]);
   } else {
@@ -88,13 +89,10 @@ __device__ __forceinline__ int tile_e(float top) {
   const int e = (int)(__float_as_uint(top) >> 23) - 126;
   return min(max(e, E_MIN), E_MAX);
 }
-// Nibble of v at tile exponent e.  The product with a power of two is exact
+// Mantissa of v at tile exponent e (up = 2^(3 - e)).  The product with a power of two is exact
 // where it matters (an underflowing one rounds to 0 anyway); the conversion
 // rounds half to even, saturates +-Inf and takes NaN to 0.
-__device__ __forceinline__ unsigned nibble(float v, float up) {
-  const int m = __float2int_rn(__fmul_rn(v, up));
-  return (unsigned)(min(max(m, -8), 7) + 8);
-}
+__device__ __forceinline__ int mantissa(float v, float up) { return min(max(__float2int_rn(__fmul_rn(v, up)), -8), 7); }
 __device__ __forceinline__ float pow2f(int k) { return __int_as_float((k + 127) << 23); }
 
 // The sequence whose tokens contain token t: the last b with q_start[b] <= t.
