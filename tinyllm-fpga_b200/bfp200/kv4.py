@@ -100,64 +100,86 @@ def new_pool(n_pages, H_KV, HD, page=64, device=None):
     return torch.empty((n_pages, H_KV, page, HD * 9 // 8), dtype=torch.uint8, device=device or torch.device("cuda"))
 
 
-def _run(fn, packed, dev):
-    """Calls a C entry point on torch's current stream of `dev`."""
-    index = dev.index
-    if torch._C._cuda_getDevice() == index:
-        rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
+def _fn(name):
+    """A C entry point of the library, looked up once."""
+    f = _fns.get(name)
+    if f is None:
+        f = _fns[name] = getattr(_lib.lib(), name)
+    return f
+
+
+_fns = {}
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or (lambda: torch.cuda.current_device())
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _run(fn, packed, index):
+    """Calls a C entry point on torch's current stream of GPU `index`."""
+    if _current_device() == index:
+        rc = fn(packed, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(packed, _raw_stream(index))
     if rc:
         check(rc)
 
 
-def _acts(x, name, dev=None, dtype=None, heads=None, hd=None, tokens=None):
-    """An activation tensor's checks; returns its shape and outer strides."""
-    if x.dim() != 3 or x.dtype not in _DTYPES or not x.is_cuda:
+def _acts(x, name):
+    """An activation tensor's GPU, dtype code, shape and outer strides."""
+    code = _DTYPES.get(x.dtype)
+    if code is None or x.dim() != 3 or not x.is_cuda:
         _bad(f"{name} must be a [tokens, heads, HD] float32, float16 or bfloat16 tensor on the GPU")
     t, h, d = x.shape
     st, sh, sd = x.stride()
     if sd != 1 and d > 1 and t and h:
         _bad(f"{name}'s last axis must be contiguous")
-    if dev is not None and x.device != dev:
+    return x.get_device(), code, t, h, d, st, sh
+
+
+def _like(x, name, dev, code, t, h, d):
+    """Outer strides of a tensor that has to fit another one."""
+    v = _acts(x, name)
+    if v[0] != dev:
         _bad(f"{name} is on another device")
-    if dtype is not None and x.dtype != dtype:
+    if v[1] != code:
         _bad(f"{name} must have the same dtype as the other tensors")
-    if (heads is not None and h != heads) or (hd is not None and d != hd) or (tokens is not None and t != tokens):
+    if v[2] != t or v[3] != h or v[4] != d:
         _bad(f"{name} has shape {tuple(x.shape)}, which does not fit the other arguments")
-    return t, h, d, st, sh
+    return v[5], v[6]
 
 
-def _ints(x, name, dev, dims):
-    if x.dtype != torch.int32 or x.dim() != dims or x.device != dev:
-        _bad(f"{name} must be an int32 tensor with {dims} axes on the same GPU")
-    return x
+def _positions(x, dev, tokens):
+    if x.dtype != torch.int32 or x.dim() != 1 or x.get_device() != dev or x.shape[0] != tokens \
+            or (tokens > 1 and x.stride(0) != 1):
+        _bad("positions must be a contiguous int32 tensor on the same GPU with one entry per token")
+    return x.data_ptr()
 
 
 def _batch(pool, q_start, lens, block_table, tokens):
-    """The 12 words of bfp200_kv4_batch."""
-    if pool.dtype != torch.uint8 or pool.dim() != 4 or not pool.is_contiguous() or not pool.is_cuda:
+    """The GPU and the 12 words of bfp200_kv4_batch."""
+    if pool.dtype != torch.uint8 or pool.dim() != 4 or not pool.is_cuda or not pool.is_contiguous():
         _bad("pool must be a contiguous uint8 [pages, H_KV, page, HD * 9 / 8] tensor on the GPU")
-    dev = pool.device
+    dev = pool.get_device()
     n_pages, h, page, rec = pool.shape
-    n = lens.shape[0] if lens.dim() == 1 else -1
-    if lens.dtype != torch.int32 or q_start.dtype != torch.int32 or block_table.dtype != torch.int32 or n < 0 \
-            or q_start.dim() != 1 or q_start.shape[0] != n + 1 or block_table.dim() != 2 or block_table.shape[0] != n:
-        _bad("lens [n], q_start [n + 1] and block_table [n, pages] must be int32 and fit each other")
-    if lens.device != dev or q_start.device != dev or block_table.device != dev:
+    if lens.dtype != torch.int32 or q_start.dtype != torch.int32 or block_table.dtype != torch.int32 \
+            or lens.dim() != 1 or q_start.dim() != 1 or block_table.dim() != 2:
+        _bad("lens [n], q_start [n + 1] and block_table [n, pages] must be int32")
+    n, width = block_table.shape
+    ld, step = block_table.stride()
+    if lens.shape[0] != n or q_start.shape[0] != n + 1:
+        _bad("lens [n], q_start [n + 1] and block_table [n, pages] must fit each other")
+    if lens.get_device() != dev or q_start.get_device() != dev or block_table.get_device() != dev:
         _bad("lens, q_start and block_table must be on the pool's device")
-    width = block_table.shape[1]
-    if (n > 1 and lens.stride(0) != 1) or q_start.stride(0) != 1 or (width > 1 and block_table.stride(1) != 1):
+    if (n > 1 and lens.stride(0) != 1) or q_start.stride(0) != 1 or (width > 1 and step != 1):
         _bad("lens, q_start and block_table's rows must be contiguous")
     if rec % 9:
         _bad("the pool's last axis must be HD * 9 / 8")
-    return (pool.data_ptr(), block_table.data_ptr(), q_start.data_ptr(), lens.data_ptr(), n_pages, page, h, rec * 8 // 9,
-            n, width, block_table.stride(0), tokens)
+    return dev, (pool.data_ptr(), block_table.data_ptr(), q_start.data_ptr(), lens.data_ptr(), n_pages, page, h,
+                 rec * 8 // 9, n, width, ld, tokens)
 
 
 def _table(table, dev):
-    if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2 or table.device != dev \
+    if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2 or table.get_device() != dev \
             or not table.is_contiguous():
         _bad("table must be a contiguous float32 [n_pos, rot / 2, 2] tensor on the same GPU")
     return table.data_ptr(), table.shape[0], table.shape[1] * 2
@@ -168,18 +190,16 @@ def rope(x, positions, table, interleaved=False, inverse=False, out=None):
     every head turned by its token's angles: pairs (j, j + rot / 2), or (2 j,
     2 j + 1) if interleaved; the other dims are copied.  inverse turns back,
     which is the gradient of the forward turn.  out may be x."""
-    t, h, d, xt, xh = _acts(x, "x")
-    dev = x.device
+    dev, code, t, h, d, xt, xh = _acts(x, "x")
     if out is None:
-        out = torch.empty((t, h, d), dtype=x.dtype, device=dev)
-    _, _, _, ot, oh = _acts(out, "out", dev, x.dtype, h, d, t)
-    _ints(positions, "positions", dev, 1)
-    if positions.shape[0] != t or (t > 1 and positions.stride(0) != 1):
-        _bad("positions must hold one entry per token")
+        out = x.new_empty((t, h, d))
+        ot, oh = h * d, d
+    else:
+        ot, oh = _like(out, "out", dev, code, t, h, d)
+    pp = _positions(positions, dev, t)
     tp, n_pos, rot = _table(table, dev)
-    _run(_lib.lib().bfp200_rope_dev,
-         _ROPE.pack(x.data_ptr(), out.data_ptr(), tp, positions.data_ptr(), xt, xh, ot, oh, t, h, d, n_pos, rot,
-                    _DTYPES[x.dtype], interleaved, inverse), dev)
+    _run(_fn("bfp200_rope_dev"), _ROPE.pack(x.data_ptr(), out.data_ptr(), tp, pp, xt, xh, ot, oh, t, h, d, n_pos, rot, code,
+                                            interleaved, inverse), dev)
     return out
 
 
@@ -189,33 +209,31 @@ def append(pool, k, v, q_start, lens, block_table, q=None, table=None, interleav
     keys and the queries q [tokens, H_Q, HD] are rotated on the way, by their
     cache positions or by `positions` [tokens].  Returns the rotated queries
     (q_out if given, which may be q), or None without q."""
-    t, h, d, kt, kh = _acts(k, "k")
-    dev, dtype = k.device, k.dtype
-    _, _, _, vt, vh = _acts(v, "v", dev, dtype, h, d, t)
-    b = _batch(pool, q_start, lens, block_table, t)
-    if pool.device != dev or b[6] != h or b[7] != d:
+    dev, code, t, h, d, kt, kh = _acts(k, "k")
+    vt, vh = _like(v, "v", dev, code, t, h, d)
+    where, b = _batch(pool, q_start, lens, block_table, t)
+    if where != dev or b[6] != h or b[7] != d:
         _bad("k and v do not fit the pool's heads, HD or device")
     hq = qt = qh = ot = oh = qp = op = tp = n_pos = rot = pp = 0
     if q is not None:
-        _, hq, _, qt, qh = _acts(q, "q", dev, dtype, None, d, t)
+        hq = q.shape[1] if q.dim() == 3 else 0
+        qt, qh = _like(q, "q", dev, code, t, hq, d)
         if q_out is None:
-            q_out = torch.empty((t, hq, d), dtype=dtype, device=dev)
-        _, _, _, ot, oh = _acts(q_out, "q_out", dev, dtype, hq, d, t)
+            q_out = q.new_empty((t, hq, d))
+            ot, oh = hq * d, d
+        else:
+            ot, oh = _like(q_out, "q_out", dev, code, t, hq, d)
         qp, op = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         _bad("q_out needs q")
     if table is not None:
         tp, n_pos, rot = _table(table, dev)
         if positions is not None:
-            _ints(positions, "positions", dev, 1)
-            if positions.shape[0] != t or (t > 1 and positions.stride(0) != 1):
-                _bad("positions must hold one entry per token")
-            pp = positions.data_ptr()
+            pp = _positions(positions, dev, t)
     elif positions is not None:
         _bad("positions need a table")
-    _run(_lib.lib().bfp200_kv4_append_dev,
-         _APPEND.pack(*b, k.data_ptr(), v.data_ptr(), qp, op, kt, kh, vt, vh, qt, qh, ot, oh, tp, pp, hq, n_pos, rot,
-                      _DTYPES[dtype], interleaved), dev)
+    _run(_fn("bfp200_kv4_append_dev"), _APPEND.pack(*b, k.data_ptr(), v.data_ptr(), qp, op, kt, kh, vt, vh, qt, qh, ot, oh, tp,
+                                                    pp, hq, n_pos, rot, code, interleaved), dev)
     return q_out
 
 
@@ -223,12 +241,15 @@ def read(pool, q_start, lens, block_table, tokens, dtype=torch.bfloat16):
     """(k, v) [tokens, H_KV, HD]: what the cache holds for the last q_start[s +
     1] - q_start[s] positions of every sequence (all of them with q_start =
     cumsum of lens).  Exact in every dtype."""
-    if dtype not in _DTYPES:
+    code = _DTYPES.get(dtype)
+    if code is None:
         _bad("dtype must be float32, float16 or bfloat16")
-    b = _batch(pool, q_start, lens, block_table, tokens)
-    k = torch.empty((tokens, b[6], b[7]), dtype=dtype, device=pool.device)
-    v = torch.empty((tokens, b[6], b[7]), dtype=dtype, device=pool.device)
-    _run(_lib.lib().bfp200_kv4_read_dev, _READ.pack(*b, k.data_ptr(), v.data_ptr(), _DTYPES[dtype]), pool.device)
+    if tokens < 0:
+        _bad("tokens must not be negative")
+    dev, b = _batch(pool, q_start, lens, block_table, tokens)
+    k = pool.new_empty((tokens, b[6], b[7]), dtype=dtype)
+    v = pool.new_empty((tokens, b[6], b[7]), dtype=dtype)
+    _run(_fn("bfp200_kv4_read_dev"), _READ.pack(*b, k.data_ptr(), v.data_ptr(), code), dev)
     return k, v
 
 
@@ -240,24 +261,24 @@ def attention(q, pool, q_start, lens, block_table, scale=None, causal=True, wind
     HD^-1/2.  Returns out, and with return_lse the log-sum-exp of the scaled
     scores (float32 [tokens, H_Q]) to join it with attention over other keys;
     a token that sees nothing gets zeros and -inf."""
-    t, hq, d, qt, qh = _acts(q, "q")
-    dev = q.device
-    b = _batch(pool, q_start, lens, block_table, t)
-    if pool.device != dev or b[7] != d:
+    dev, code, t, hq, d, qt, qh = _acts(q, "q")
+    where, b = _batch(pool, q_start, lens, block_table, t)
+    if where != dev or b[7] != d:
         _bad("q does not fit the pool's HD or device")
     if out is None:
-        out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
-    _, _, _, ot, oh = _acts(out, "out", dev, q.dtype, hq, d, t)
-    L = _lib.lib()
-    lse = torch.empty((t, hq), dtype=torch.float32, device=dev) if return_lse else None
-    words = (*b, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0)
-    tail = (qt, qh, ot, oh, hq, _DTYPES[q.dtype], causal, window, d ** -0.5 if scale is None else scale)
-    need = _workspace_bytes.get((dev.index, d))
+        out = q.new_empty((t, hq, d))
+        ot, oh = hq * d, d
+    else:
+        ot, oh = _like(out, "out", dev, code, t, hq, d)
+    lse = q.new_empty((t, hq), dtype=torch.float32) if return_lse else None
+    need = _workspace_bytes.get((dev, d))
     if need is None:
         n = _lib.C.c_size_t()
         with torch.cuda.device(dev):
-            check(L.bfp200_kv4_attention_workspace(_ATTENTION.pack(*words, 0, 0, *tail), _lib.C.byref(n)))
-        need = _workspace_bytes[(dev.index, d)] = n.value
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _run(L.bfp200_kv4_attention_dev, _ATTENTION.pack(*words, ws.data_ptr(), need, *tail), dev)
+            check(_fn("bfp200_kv4_attention_workspace")(_ATTENTION.pack(*b, *[0] * 9, hq, code, 0, 0, 0.0), _lib.C.byref(n)))
+        need = _workspace_bytes[(dev, d)] = n.value
+    ws = q.new_empty((need,), dtype=torch.uint8)
+    _run(_fn("bfp200_kv4_attention_dev"),
+         _ATTENTION.pack(*b, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, ws.data_ptr(), need, qt, qh, ot, oh,
+                         hq, code, causal, window, d ** -0.5 if scale is None else scale), dev)
     return (out, lse) if return_lse else out

@@ -22,6 +22,7 @@
 // pairs of an operand whose contraction axis is the position.  No two
 // positions share a byte, so tokens of one page may be written concurrently.
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -116,6 +117,17 @@ __device__ __forceinline__ int find_seq(const int* q_start, int n_seq, int t) {
 __device__ __forceinline__ long long record_of(const Batch& b, int seq, int pos, int head, int rec_bytes) {
   const int pg = __ldg(b.bt + (long long)seq * b.bt_ld + (pos >> b.page_shift));
   return (unsigned)pg < (unsigned)b.n_pages ? ((long long)pg * b.H + head) * rec_bytes : -1;
+}
+
+// Dynamic shared memory of a kernel on the current device, raised once.
+template <typename K>
+cudaError_t allow_smem(K* kern, size_t bytes, std::atomic<unsigned char> (&done)[128]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || done[dev].load(std::memory_order_relaxed)) return e;   // (device_ready keeps dev below 128)
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done[dev].store(1, std::memory_order_relaxed);
+  return e;
 }
 
 int fill_batch(const bfp200_kv4_batch& in, Batch* out, const char* who);   // BFP200_OK or the error of the calling thread

@@ -661,11 +661,9 @@ cudaError_t launch_attn(AttnArgs a, int n_sm, float* ws, cudaStream_t s) {
   constexpr size_t smem = SH::template smem<Kind<T>::QS>();
   static_assert(smem + 2048 <= 227 * 1024, "shared memory");
   auto* kern = attn_kernel<T, HD, NT>;
-  cudaError_t e;
-  if (smem > 40 * 1024) {                                          // static shared memory counts, too
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
+  static std::atomic<unsigned char> allowed[128];
+  cudaError_t e = allow_smem(kern, smem, allowed);
+  if (e != cudaSuccess) return e;
   a.grid = n_sm * SH::CTAS;
   a.cuts = reinterpret_cast<Cut*>(ws);
   a.part = reinterpret_cast<float*>(a.cuts + a.grid);

@@ -737,7 +737,8 @@ size_t prompt_ws_bytes(int hd, int n_sm) { return (size_t)n_sm * (sizeof(Cut) + 
 template <typename T, int HD>
 cudaError_t launch_prompt(AttnArgs a, int n_sm, float* ws, cudaStream_t s) {
   auto* kern = prompt_kernel<T, HD>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM<HD>);
+  static std::atomic<unsigned char> allowed[128];
+  cudaError_t e = allow_smem(kern, SMEM<HD>, allowed);
   if (e != cudaSuccess) return e;
   int* err = error_flag_device_ptr();
   if (!err) return cudaErrorInvalidSymbol;
