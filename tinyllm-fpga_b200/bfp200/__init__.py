@@ -18,6 +18,9 @@ engine   Decoder (one GPU), generate_multi (sequence-parallel, no collectives),
 dist     one process per GPU: step-balanced sequence partition, token gather,
          sharded-head argmax exchange (torch.distributed)
 sim      drop-in facade with the reference module's names
+kv4      rotary positions and a paged KV cache held in 4 bits (append, read,
+         attention) on torch tensors (needs torch)
+paged    batched greedy generation over that cache
 """
 from ._lib import BfpError
 from .config import BfpConfig, SMOLLM2_135M
