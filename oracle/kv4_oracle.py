@@ -40,6 +40,18 @@ def put(rec, slot, page, k, v):
         rec[ex[0::16]] = e + 18
 
 
+def put_pages(pool, k, v):
+    """Whole pages: float keys and values [n, H, page, HD] into records pool [n, H, record] (uint8)."""
+    page, HD = k.shape[2:]
+    for x, which in ((k, 0), (v, 1)):
+        m, e = quantize(x)
+        n = (m + 8).astype(np.uint8)
+        for slot in range(page):
+            at, ex = addresses(slot, page, HD)[which], addresses(slot, page, HD)[2 + which]
+            pool[..., at[0::2]] = n[:, :, slot, 0::2] | (n[:, :, slot, 1::2] << 4)
+            pool[..., ex[0::16]] = e[:, :, slot] + 18
+
+
 def get(rec, slot, page, HD):
     kb, vb, ke, ve = addresses(slot, page, HD)
     sh = np.where(np.arange(HD) % 2, 4, 0)

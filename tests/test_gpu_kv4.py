@@ -363,6 +363,34 @@ def test_attention_long_axis_is_split(dtype, new):
     _attend(case, _rand(rng, (new, 3, 64), dtype), dtype, window=3001)
 
 
+@pytest.mark.parametrize("HD,page", [(64, 64), (128, 16)])
+def test_attention_many_prompt_items(HD, page):
+    """More items than CTAs, of one and of two tiles of 128 rows in turn, cut
+    anywhere, with causal tiles of different lengths."""
+    import torch
+    rng = np.random.default_rng(HD)
+    n, H, G = 48, 5, 3
+    lens, news = rng.integers(100, 600, n), rng.integers(40, 100, n)
+    used = [-(-int(L) // page) for L in lens]
+    pool = np.full((sum(used), H, page * HD * 9 // 8), 0xFF, np.uint8)
+    k, v = rng.standard_normal((2, sum(used), H, page, HD))
+    O.put_pages(pool, k, v)
+    case = Case.__new__(Case)
+    case.lens, case.news, case.HD, case.page = [int(x) for x in lens], [int(x) for x in news], HD, page
+    bt = np.full((n, max(used)), -1)
+    first = np.concatenate([[0], np.cumsum(used)])
+    case.kv = []
+    for s in range(n):
+        bt[s, :used[s]] = np.arange(first[s], first[s + 1])
+        flat = lambda x: O.value(*O.quantize(x[first[s]:first[s + 1]].transpose(0, 2, 1, 3).reshape(-1, H, HD)[:lens[s]]))
+        case.kv.append((flat(k), flat(v)))
+    case.bt, case.len_t, case.q_start = _i32(bt), _i32(lens), _i32(np.concatenate([[0], np.cumsum(news)]))
+    case.pool = torch.from_numpy(pool.reshape(-1, H, page, HD * 9 // 8)).cuda()
+    q = _rand(rng, (int(news.sum()), H * G, HD), "bfloat16")
+    _attend(case, q, "bfloat16")
+    _attend(case, q, "bfloat16", window=150)
+
+
 def test_attention_many_sequences():
     rng = np.random.default_rng(77)
     lens = rng.integers(0, 90, 700)

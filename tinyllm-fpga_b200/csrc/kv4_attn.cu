@@ -43,10 +43,13 @@ namespace {
 // work (addresses, waits, the test of the maximum) is shared by more values.
 template <int HD> constexpr int SUB = HD <= 64 ? 2 : 1;
 template <int HD> constexpr int BLK_OF = 32 * SUB<HD>;
-constexpr int MINB = 8;            // blocks that are not worth a second CTA
+constexpr int MINB = 4;            // blocks that are not worth a second CTA: one for each warp
+// An item's fixed cost (its queries, first loads and joining) in blocks, for
+// the cuts (256 sequences of up to 2047, 9 / 3 heads of 64: 41.7 us at 0, 36.2 at 4).
+constexpr int ITEM = 4;
 // ---- the split ---------------------------------------------------------------
 struct Seq {
-  int q0, n_q, len, blk0, nb, rt;  // first token, tokens, positions, first block, blocks, row tiles
+  int q0, n_q, len, blk0, nb, rt;  // first token, tokens, positions, first block, blocks plus ITEM, row tiles
 };
 
 // Blocks before each sequence (or chunk of `per` sequences, where there are
@@ -69,7 +72,7 @@ __device__ __forceinline__ Seq seq_make(const AttnArgs& a, int q0, int n_q, int 
   r.len = len;
   const long long first = a.window ? (long long)len - n_q - a.window + 1 : 0;
   r.blk0 = first > 0 ? min((int)(first / BLK), max(len - 1, 0) / BLK) : 0;
-  r.nb = max((len + BLK - 1) / BLK - r.blk0, 1);
+  r.nb = max((len + BLK - 1) / BLK - r.blk0, 1) + ITEM;
   const long long rows = (long long)n_q * a.group;
   r.rt = (int)((rows + NR - 1) / NR);
   return r;
@@ -127,7 +130,7 @@ __device__ void make_sched(const AttnArgs& a, Sched& s) {
     s.pre[SCH] = total;
     s.total = total;
     s.geff = max(min((long long)a.grid, max(n_items, (total + MINB - 1) / MINB)), 1LL);
-    s.delta = max(total / (s.geff * 32), (long long)(MINB / 2));
+    s.delta = max(total / (s.geff * 32), (long long)(ITEM + 1));   // no cut leaves less than a block
     s.per = per;
   }
   __syncthreads();
@@ -310,8 +313,9 @@ __global__ void __launch_bounds__(Shape<HD, NT>::W * 32, Shape<HD, NT>::CTAS) at
     __syncthreads();
 
     // this segment's blocks that some row sees, as positions
-    const int first = max((int)(x - it.start) + it.q.blk0, any_lo / BLK);
-    const int last = min((int)(xe - it.start) + it.q.blk0, (any_hi + BLK - 1) / BLK);
+    const int skip = x == it.start ? 0 : (int)(x - it.start) - ITEM;   // blocks of CTAs before this one
+    const int first = max(skip + it.q.blk0, any_lo / BLK);
+    const int last = min((int)(xe - it.start) - ITEM + it.q.blk0, (any_hi + BLK - 1) / BLK);
     const int* bt = a.b.bt + (long long)it.seq * a.b.bt_ld;
     const auto page_at = [&](int pos) -> int {
       const int i = pos >> a.b.page_shift;

@@ -26,7 +26,9 @@ namespace {
 constexpr int PR = 256, PB = 128;            // rows of an item, positions of a block (of keys and values in shared memory)
 constexpr int PU = 64;                       // positions of a unit: one MMA group of scores, one softmax step
 constexpr int MIN_SHARE = 8;                 // blocks that are not worth a second CTA
-constexpr int ITEM = 3;                      // an item's queries, first block and outputs, in blocks
+// An item's queries, first block and outputs, in blocks (8192 tokens, 32 / 8
+// heads of 128: 730 us at 3, 646 at 6, 666 at 9).
+constexpr int ITEM = 6;
 constexpr int THREADS = 512;                  // softmax 2 x 4 warps, decoding 4, MMA 2 (and 2 that wait at the end)
 constexpr int SPIN = 1 << 20;
 
@@ -83,7 +85,7 @@ __device__ __forceinline__ void ld32(uint32_t at, uint32_t* r) {
                  "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                : "r"(at) : "memory");
 }
-__device__ __forceinline__ void st32(uint32_t at, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void st32(uint32_t at, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
                "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
                :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
@@ -92,17 +94,6 @@ __device__ __forceinline__ void st32(uint32_t at, const uint32_t (&r)[32]) {
                   "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]),
                   "r"(at) : "memory");
 }
-__device__ __forceinline__ void st_n(uint32_t at, const uint32_t (&r)[16]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
-               :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                  "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-                  "r"(at) : "memory");
-}
-__device__ __forceinline__ void st_n(uint32_t at, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};"
-               :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(at) : "memory");
-}
-
 // ---- the split: as in kv4_attn.cu, but under a causal mask or a window every
 // row tile has its own number of blocks.  The functions are a warp's.
 constexpr int CH = 256;
@@ -305,10 +296,10 @@ __device__ __forceinline__ void hide(uint32_t (&s)[N], int at, int lo, int hi) {
   for (int k = 0; k < N; ++k) s[k] = at + k < hi && at + k >= lo ? s[k] : 0xFF800000u;
 }
 
-// P = ex2(scale s - ref) of a row's 64 scores, written over them in tensor
-// memory as MMA operand; returns their sum.
+// P = ex2(scale s - ref) of a row's 64 scores, as MMA operand (of every 16
+// columns the 8 words, then the 8 of its low part); returns their sum.
 template <int PS>
-__device__ __forceinline__ float row_weights(uint32_t tS, const uint32_t (&s)[64], float scale, float ref) {
+__device__ __forceinline__ float row_weights(uint32_t (&ph)[32 * PS], const uint32_t (&s)[64], float scale, float ref) {
   const uint64_t sl = pack2(scale, scale), rf = pack2(-ref, -ref);
   uint64_t add[2] = {0, 0};
   #pragma unroll
@@ -321,18 +312,16 @@ __device__ __forceinline__ float row_weights(uint32_t tS, const uint32_t (&s)[64
       p[k + 1] = ex2(y.y);
       add[(k >> 1) & 1] = add2(add[(k >> 1) & 1], pack2(p[k], p[k + 1]));
     }
-    uint32_t ph[8 * PS];                                    // of 16 columns: the operand, then its low part
     #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int ia = (k >> 2) * 8 + (k & 3), ib = ia + 4;
       const __half2 h = __floats2half2_rn(p[ia], p[ib]);
-      ph[k] = as_u(h);
+      ph[c * 8 * PS + k] = as_u(h);
       if constexpr (PS == 2) {
         const float2 back = __half22float2(h);
-        ph[8 + k] = as_u(__floats2half2_rn(p[ia] - back.x, p[ib] - back.y));
+        ph[c * 16 + 8 + k] = as_u(__floats2half2_rn(p[ia] - back.x, p[ib] - back.y));
       }
     }
-    st_n(tS + c * 8 * PS, ph);
   }
   const float2 t0 = unpack2(add[0]), t1 = unpack2(add[1]);
   return (t0.x + t0.y) + (t1.x + t1.y);
@@ -435,20 +424,25 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
         const int blocks0 = tile ? g.nt1 : g.nk, seg = tile ? g.seg1 : g.seg0;
         // queries: [dim / 8][row][dims 0 4 1 5 2 6 3 7]
         const T* q = static_cast<const T*>(a.q) + (long long)(q0 + j) * a.q_ts + (long long)head * a.q_hs;
-        #pragma unroll 4
-        for (int c = 0; c < HD / 8; ++c) {
-          uint4 v = make_uint4(0, 0, 0, 0);
+        uint4 qv[HD / 8];
+        #pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {                  // (all of the row's loads at once)
+          qv[c] = make_uint4(0, 0, 0, 0);
           if (live) {
             if (q_vec) {
-              v = __ldg(reinterpret_cast<const uint4*>(q + c * 8));
+              qv[c] = __ldg(reinterpret_cast<const uint4*>(q + c * 8));
             } else {
               unsigned short e[8];
               #pragma unroll
               for (int i = 0; i < 8; ++i) e[i] = __ldg(reinterpret_cast<const unsigned short*>(q) + c * 8 + i);
-              v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+              qv[c] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
             }
-            v.x ^= a.q_flip; v.y ^= a.q_flip; v.z ^= a.q_flip; v.w ^= a.q_flip;
           }
+        }
+        #pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          uint4 v = qv[c];
+          v.x ^= a.q_flip; v.y ^= a.q_flip; v.z ^= a.q_flip; v.w ^= a.q_flip;
           *reinterpret_cast<uint4*>(s_q + tile * TILE_Q + c * 2048 + row * 16) =
               make_uint4(prmt(v.x, v.z, 0x5410), prmt(v.x, v.z, 0x7632), prmt(v.y, v.w, 0x5410), prmt(v.y, v.w, 0x7632));
         }
@@ -471,6 +465,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
           ld32(tU + 32, s + 32);
           wait_ld();
           if (!whole) hide(s, base, lo, hi);
+          // The weights by the present reference, beside the maximum that tells
+          // whether it still serves (one unit in many it does not).
+          uint32_t ph[32 * PS];
+          float sum = row_weights<PS>(ph, s, a.scale_log2, ref);
           float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           #pragma unroll
           for (int k = 0; k < PU; k += 2) top[(k >> 1) & 3] = fmaxf(top[(k >> 1) & 3], fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 1])));
@@ -495,8 +493,11 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
                 st32(tO + c * 32, o);
               }
             }
+            sum = row_weights<PS>(ph, s, a.scale_log2, ref);
           }
-          l += row_weights<PS>(tU, s, a.scale_log2, ref);
+          l += sum;
+          st32(tU, ph);
+          if constexpr (PS == 2) st32(tU + 32, ph + 32);
           wait_st();
           tc_before();
           __syncwarp();
@@ -665,7 +666,17 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
     if (warp < 14) share([&](const Seg& g) {
       const int n = g.n, nk = g.nk, t = warp - 12;
       const bool both = g.rows > 128;
-      if (t && !both) return;
+      if (t && !both) {
+        // No tile of its own: it still gives back every block, so that it is never
+        // ahead of the phases that it will wait for in a later item.
+        for (int kc = nk; kc < nk + n; ++kc) {
+          if (!(ok = warp_wait(&kfull[kc & 1], (kc >> 1) & 1))) return;
+          if (lane == 0) mb_arrive(&kfree[kc & 1]);
+          if (!(ok = warp_wait(&vfull[kc & 1], (kc >> 1) & 1))) return;
+          if (lane == 0) mb_arrive(&vfree[kc & 1]);
+        }
+        return;
+      }
       constexpr uint32_t i_qk = idesc_f16(HALF_K ? 0 : 1, 128, PU), i_pv = idesc_f16(0, 128, HD);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t tS = tm + t * 128, tO = tm + 256 + t * HD;
@@ -679,16 +690,12 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
           mma_ss(tS + (u & 1) * PU, dq + k * 256, dk + st * (TILE_KV >> 4) + (u & 1) * (PU * 16 >> 4) + k * 256, i_qk, k > 0);
         tc_commit(&sfull[t][u & 1]);
       };
-      const auto free = [&](unsigned long long* bar) {      // two arrivals, one of each tile that there is
-        tc_commit(bar);
-        if (!both) tc_commit(bar);
-      };
       ok = warp_wait(&qfull[t], (t ? g.seg1 : g.seg0) & 1) && warp_wait(&kfull[nk & 1], (nk >> 1) & 1);
       tc_after();
       if (ok && elect_one()) {
         scores(0, nk & 1);
         scores(1, nk & 1);
-        free(&kfree[nk & 1]);
+        tc_commit(&kfree[nk & 1]);                          // (two arrivals, one of each MMA warp)
       }
       __syncwarp();
       for (int u = 0; u < 2 * n && ok; ++u) {
@@ -708,8 +715,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
           if (more) scores(u, st ^ 1);
           else tc_commit(&ofull[t][u & 1]);                 // the last two units'
           if (u & 1) {
-            free(&vfree[st]);
-            if (more) free(&kfree[st ^ 1]);
+            tc_commit(&vfree[st]);
+            if (more) tc_commit(&kfree[st ^ 1]);
           }
         }
         __syncwarp();
