@@ -124,6 +124,17 @@ def _run(fn, packed, index):
         check(rc)
 
 
+def _workspace(packed, index):
+    n = _lib.C.c_size_t()
+    f = _fn("bfp200_kv4_attention_workspace")
+    if _current_device() == index:
+        check(f(packed, n))
+    else:
+        with torch.cuda.device(index):
+            check(f(packed, n))
+    return n.value
+
+
 def _acts(x, name):
     """An activation tensor's GPU, dtype code, shape and outer strides."""
     code = _DTYPES.get(x.dtype)
@@ -271,14 +282,14 @@ def attention(q, pool, q_start, lens, block_table, scale=None, causal=True, wind
     else:
         ot, oh = _like(out, "out", dev, code, t, hq, d)
     lse = q.new_empty((t, hq), dtype=torch.float32) if return_lse else None
-    need = _workspace_bytes.get((dev, d))
+    small = b[5] * b[9] <= 256                  # a cache that short may need none: asked for each time
+    need = None if small else _workspace_bytes.get((dev, d))
     if need is None:
-        n = _lib.C.c_size_t()
-        with torch.cuda.device(dev):
-            check(_fn("bfp200_kv4_attention_workspace")(_ATTENTION.pack(*b, *[0] * 9, hq, code, 0, 0, 0.0), _lib.C.byref(n)))
-        need = _workspace_bytes[(dev, d)] = n.value
-    ws = q.new_empty((need,), dtype=torch.uint8)
+        need = _workspace(_ATTENTION.pack(*b, 0, 0, 0, 0, 0, 0, 0, 0, 0, hq, code, 0, 0, 0.0), dev)
+        if not small:
+            _workspace_bytes[(dev, d)] = need
+    ws = q.new_empty((need,), dtype=torch.uint8) if need else None
     _run(_fn("bfp200_kv4_attention_dev"),
-         _ATTENTION.pack(*b, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, ws.data_ptr(), need, qt, qh, ot, oh,
+         _ATTENTION.pack(*b, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, ws.data_ptr() if need else 0, need, qt, qh, ot, oh,
                          hq, code, causal, window, d ** -0.5 if scale is None else scale), dev)
     return (out, lse) if return_lse else out

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::W * 32, Shape<HD, NT>::CTAS) at
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   make_sched<NR, BLK, W * 32>(a, sch);
-  if (tid == 0) a.cuts[blockIdx.x].parts = 0;
+  if (tid == 0 && a.cuts) a.cuts[blockIdx.x].parts = 0;
   if ((long long)blockIdx.x >= sch.geff || sch.total == 0) return;
   long long x = bound<NR, BLK>(a, sch, (long long)blockIdx.x + (lane & 1));   // both bounds at once
   const long long x1 = __shfl_sync(0xffffffffu, x, 1);
@@ -658,6 +658,11 @@ __global__ void __launch_bounds__(Shape<HD, NT>::W * 32, Shape<HD, NT>::CTAS) at
   }
 }
 
+// Items of at most MINB blocks are never cut: an edge lies within ITEM + 1 of
+// every place in them.  No workspace then, and no joining launch.
+template <int HD> bool never_cut(const Batch& b) { return (long long)b.max_pages * b.page <= MINB * BLK_OF<HD>; }
+static_assert(MINB + ITEM <= 2 * (ITEM + 1), "items of MINB blocks stay whole");
+
 template <typename T, int HD, int NT>
 cudaError_t launch_attn(AttnArgs a, int n_sm, float* ws, cudaStream_t s) {
   using SH = Shape<HD, NT>;
@@ -669,23 +674,29 @@ cudaError_t launch_attn(AttnArgs a, int n_sm, float* ws, cudaStream_t s) {
   cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
   a.grid = n_sm * SH::CTAS;
-  a.cuts = reinterpret_cast<Cut*>(ws);
-  a.part = reinterpret_cast<float*>(a.cuts + a.grid);
+  const bool whole = never_cut<HD>(a.b);
+  a.cuts = whole ? nullptr : reinterpret_cast<Cut*>(ws);
+  a.part = whole ? nullptr : reinterpret_cast<float*>(a.cuts + a.grid);
   kern<<<a.grid, W * 32, smem, s>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  // items of at most MINB blocks are never cut
-  if ((long long)a.b.max_pages * a.b.page <= MINB * BLK_OF<HD>) return cudaSuccess;
+  if (whole) return cudaSuccess;
   return launch_join<T, HD, NR>(a, 4, s);
 }
 
-// Row tile of a call: the sequences' average of tokens times the group.
-int pick_nt(const Batch& b, int group, bool wide) {
+// Row tile of a call, by the sequences' average of tokens times the group; 8
+// stands for the prompt kernel.  At heads of 128 it is ahead from 64 rows on (16
+// sequences of up to 4000 positions, 24 tokens of 32 / 8 heads: 82 us against 123),
+// at 64 and fewer dims, where decoding is half and the softmax all of the work,
+// from some 300 (100 tokens of 9 / 3 heads: 90 against 96; 48 tokens: 66 against 57).
+// 32-bit queries would not fit its shared memory.
+int pick_nt(const Batch& b, int group, int hd, bool wide) {
   const long long rows = ((long long)b.T + b.n_seq - 1) / b.n_seq * group;
-  return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 || wide ? 4 : 8;
+  return rows <= 8 ? 1 : rows <= 16 ? 2 : wide || rows <= (hd > 64 ? 32 : 256) ? 4 : 8;
 }
-// Room for the partial sums of any call with this head dim.
-size_t ws_bytes(int hd, int n_sm) {
+// Room for the partial sums of any call with this head dim; none where nothing is cut.
+size_t ws_bytes(const Batch& b, int hd, int nt, int n_sm) {
+  if (nt != 8 && (hd > 64 ? never_cut<128>(b) : never_cut<64>(b))) return 0;
   size_t most = 0;
   for (int nt = 1; nt <= 4; nt *= 2) {
     const size_t grid = (size_t)n_sm * 4, b = grid * (sizeof(Cut) + 2 * nt * 8 * (hd + 2) * 4);
@@ -726,7 +737,8 @@ extern "C" int bfp200_kv4_attention_workspace(const bfp200_kv4_attention_args* i
   if (in->H_Q < 1 || in->H_Q % b.H) return bad("H_Q must be a positive multiple of H_KV");
   int n_sm = 0;
   if (int rc = device_ready(who, &n_sm)) return rc;
-  *bytes = ws_bytes((int)in->batch.HD, n_sm);
+  const int hd = (int)in->batch.HD;
+  *bytes = b.T == 0 || b.n_seq == 0 ? 0 : ws_bytes(b, hd, pick_nt(b, (int)in->H_Q / b.H, hd, in->dtype == BFP200_F32), n_sm);
   return BFP200_OK;
 }
 
@@ -763,8 +775,9 @@ extern "C" int bfp200_kv4_attention_dev(const bfp200_kv4_attention_args* in, voi
   a.q_flip = r.scale < 0 ? 0x80008000u : 0u;
   a.grid = 0;
   a.part = nullptr;
-  const int nt = pick_nt(a.b, a.group, r.dtype == BFP200_F32), hd = (int)r.batch.HD;
-  if (!r.workspace_dev || r.workspace_bytes < (long long)ws_bytes(hd, n_sm))
+  const int hd = (int)r.batch.HD, nt = pick_nt(a.b, a.group, hd, r.dtype == BFP200_F32);
+  const size_t need = ws_bytes(a.b, hd, nt, n_sm);
+  if (need && (!r.workspace_dev || r.workspace_bytes < (long long)need))
     return bad("the workspace is smaller than bfp200_kv4_attention_workspace says");
   float* ws = static_cast<float*>(r.workspace_dev);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
