@@ -1,6 +1,6 @@
 // kv4.cuh -- the 4-bit paged KV cache: record layout, tile arithmetic, batch
-// description shared by kv4.cu (rope, append, read) and kv4_attn.cu
-// (attention).
+// description shared by kv4.cu (rope, append, read), kv4_attn.cu and
+// kv4_prompt.cu (attention).
 //
 // Number format.  The framework's tiles of 16 elements with one exponent
 // (tile_quantize, gen_smollm_blockfp_full.py:90-97), with 4-bit mantissas:
@@ -110,13 +110,6 @@ __device__ __forceinline__ int find_seq(const int* q_start, int n_seq, int t) {
     lo += k * step;
   }
   return lo;
-}
-
-// Byte offset of the record of (page table slot pos / page, head), or -1 if
-// the table's entry is no page of the pool.
-__device__ __forceinline__ long long record_of(const Batch& b, int seq, int pos, int head, int rec_bytes) {
-  const int pg = __ldg(b.bt + (long long)seq * b.bt_ld + (pos >> b.page_shift));
-  return (unsigned)pg < (unsigned)b.n_pages ? ((long long)pg * b.H + head) * rec_bytes : -1;
 }
 
 // Dynamic shared memory of a kernel on the current device, raised once.

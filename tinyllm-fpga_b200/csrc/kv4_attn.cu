@@ -8,18 +8,30 @@
 // The rows of one KV head (its query heads times the call's tokens) share
 // every cached byte.  Both products run on mma.sync with the cache as the A
 // operand and the rows as N: S^T[position][row] = K Q^T and O^T[dim][row] =
-// V^T P^T, so that a group of up to 8 rows needs no padding to 16, and the
-// cache goes from global memory to the A registers without shared memory:
-// the record layout is the register layout (4 positions x 8 dims and 8
-// positions x 4 dims of 16 bytes).  S^T's accumulators become P^T's operand by
+// V^T P^T, so that a group of up to 8 rows needs no padding to 16.  A lane's
+// 16 bytes (4 positions x 8 dims, 8 positions x 4 dims) decode into A registers
+// without exchange.  Each warp fetches its blocks with cp.async into its own
+// ring in shared memory, consecutive lanes consecutive 16 bytes: a lane's own
+// units lie 64 bytes apart, and fetched straight to registers every sector
+// crossed L2 twice.  S^T's accumulators become P^T's operand by
 // one 8x8 transpose (movmatrix) per 8 positions.
 //
 // Rounding.  K is exact in the operand type; Q is split into as many operands
 // of that type as hold all its bits (1 for 16-bit types, 3 bfloat16 for
-// 32-bit); V and P use binary16, in which V 2^-4 is exact and P = 2^15 exp(s
-// - max) keeps 11 bits (bfloat16 results: an error of 2^-12 beside the
-// result's own 2^-9), or 22 bits in two operands where the result is binary16
-// or 32-bit.  Scores, maxima, sums and accumulators are 32-bit.
+// 32-bit); V and P use binary16, in which V 2^-4 is exact and P = 2^P_EXP
+// exp(s - max) (room for a maximum that is behind) keeps 11 bits (bfloat16
+// results: an error of 2^-12 beside the result's own 2^-9), or 22 bits in two
+// operands where the result is binary16 or 32-bit.  Scores, maxima, sums and
+// accumulators are 32-bit.
+//
+// What bounds it.  The cache is read once (ncu: 321 MB for 320), but a
+// pair of cached values takes 5.5 thread instructions, most of them decoding: at
+// 64 sequences of up to 8191 positions, 32 / 8 heads of 128, 58% of the issue
+// slots and 53% of the ALU are taken while the cache comes at 3.7 TB/s (87 us; 49
+// at the measured copy bandwidth), with 12 warps an SM.  Short or few sequences
+// are bound by the chain of one item (lengths, page, first block, joining): 256
+// sequences of up to 2047, 9 / 3 heads of 64, take 35 us where the bytes take 10;
+// a call for one sequence of 176 takes 14 us, launches included.
 //
 // Work split.  All (sequence, KV head, row tile) items are laid end to end in
 // blocks of 32 positions and cut evenly over the CTAs on the device, from the
