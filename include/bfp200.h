@@ -391,9 +391,9 @@ typedef struct bfp200_kv4_attention_args {
  * (causal) and k > p - window (window > 0); one that sees none gives zeros and
  * -inf. */
 int bfp200_kv4_attention_dev(const bfp200_kv4_attention_args* args, void* stream);
-/* Bytes of workspace that the call needs: 0 where max_pages * page is at most
- * 128 (256 for HD <= 64) and the call is no prompt, else the same for every
- * call of a head dim (some 40 MB at most). */
+/* Bytes of workspace that the call needs: 0 without tokens or sequences, and
+ * where max_pages * page is at most 128 (256 for HD <= 64) and the call is no
+ * prompt; else the same for every call of a head dim (some 40 MB at most). */
 int bfp200_kv4_attention_workspace(const bfp200_kv4_attention_args* args, size_t* bytes);
 
 /* Stage dump layout of bfp200_fwd_layer (mirrors the N1..D dumps of

@@ -1,0 +1,76 @@
+"""What bfp200.kv4 does with calls at the edges of its contract, on the GPU:
+empty calls, lengths past the table, rows of no sequence, calls without
+sequences.  Outputs are filled with NaN beforehand, so that a row that nobody
+writes shows.  Attention is held to the tolerance that tests/test_gpu_kv4.py
+derives."""
+import contextlib
+
+import numpy as np
+import pytest
+
+from oracle import kv4_oracle as O
+from test_gpu_kv4 import Case, DTYPES, U_OUT, U_P, _dt, _f32, _f64, _i32, _rand, _rounded
+
+pytestmark = pytest.mark.gpu
+
+
+@contextlib.contextmanager
+def _empty_is_nan():
+    """Fresh memory from torch's allocator holds NaN (bytes: 255)."""
+    import torch
+    torch.use_deterministic_algorithms(True)
+    try:
+        assert torch.utils.deterministic.fill_uninitialized_memory
+        assert torch.empty((3,), device="cuda").isnan().all()
+        yield
+    finally:
+        torch.use_deterministic_algorithms(False)
+
+
+def _visible(pos, n_keys, causal, window):
+    """[len(pos), n_keys]: what tokens at positions `pos` see of positions 0 .. n_keys - 1."""
+    p, k = np.asarray(pos)[:, None], np.arange(n_keys)[None]
+    see = (p >= 0) & (k >= 0)
+    if causal:
+        see = see & (k <= p)
+    if window:
+        see = see & (k > p - window)
+    return see
+
+
+def _check_rows(q, k, v, see, out, lse, dtype):
+    """Rows of one sequence against the formula."""
+    HD = q.shape[-1]
+    want, wl, mag = O.attention(_f64(q), k, v, see, HD ** -0.5)
+    on, ln = _f64(out), _f64(lse)
+    V = np.abs(v).max() if len(v) else 0.0
+    ds = (HD + 8) * 2.0 ** -23 * mag + 2.0 ** -21 + len(k) * 2.0 ** -24
+    tol = 2 * (ds + U_P[dtype])[..., None] * V
+    tol = tol + U_OUT[dtype] * (np.abs(want) + tol) + (2.0 ** -25 if dtype == "float16" else 0.0)
+    assert (np.abs(on - want) <= tol).all(), np.abs(on - want).max()
+    dead = np.isinf(wl)
+    assert np.array_equal(dead, np.isinf(ln)) and (ln[dead] < 0).all() and (on[dead] == 0).all()
+    assert (np.abs(ln[~dead] - wl[~dead]) <= ds[~dead] + 2.0 ** -22 * np.abs(wl[~dead])).all()
+
+
+# (HD, query heads a KV head, tokens a sequence): single tokens and few rows on
+# one kernel; more than 32 rows a sequence at heads of 128, or 256 at heads of
+# 64, on the prompts' kernel where the type has 16 bits
+FORMS = [(64, 3, 1), (64, 8, 4), (128, 8, 12), (64, 8, 40)]
+
+
+@pytest.mark.parametrize("n_seq", [0, 2])
+def test_attention_after_an_empty_call(n_seq):
+    """A call without tokens asks for no workspace; the next call still gets its own."""
+    import torch
+    from bfp200 import kv4
+    rng = np.random.default_rng(0)
+    case = Case(rng, [700], [1], 1, 64, 16)
+    kv4._workspace_bytes.clear()
+    q = torch.empty((0, 3, 64), device="cuda")
+    bt = torch.zeros((n_seq, 60), dtype=torch.int32, device="cuda")
+    out, lse = kv4.attention(q, case.pool, _i32([0] * (n_seq + 1)), _i32([500] * n_seq), bt, return_lse=True)
+    assert out.shape == (0, 3, 64) and lse.shape == (0, 3)
+    q = _rand(rng, (1, 3, 64), "float32")
+    out, lse = kv4.attention(q, case.pool, case.q_start, case.len_t, case.bt, return_lse=True)
+    _check_rows(q, *case.kv[0], _visible([699], 700, True, 0), out, lse, "float32")

@@ -283,8 +283,8 @@ def attention(q, pool, q_start, lens, block_table, scale=None, causal=True, wind
         ot, oh = _like(out, "out", dev, code, t, hq, d)
     lse = q.new_empty((t, hq), dtype=torch.float32) if return_lse else None
     small = b[5] * b[9] <= 256                  # a cache that short may need none: asked for each time
-    need = None if small else _workspace_bytes.get((dev, d))
-    if need is None:
+    need = 0 if not t or not b[8] else None if small else _workspace_bytes.get((dev, d))
+    if need is None:                            # (an empty call needs none, which says nothing of the next one)
         need = _workspace(_ATTENTION.pack(*b, 0, 0, 0, 0, 0, 0, 0, 0, 0, hq, code, 0, 0, 0.0), dev)
         if not small:
             _workspace_bytes[(dev, d)] = need
