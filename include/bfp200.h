@@ -389,7 +389,9 @@ typedef struct bfp200_kv4_attention_args {
 /* Softmax attention of the call's tokens over their sequences' cached
  * positions.  A token at position p sees the positions k < lens[s] with k <= p
  * (causal) and k > p - window (window > 0); one that sees none gives zeros and
- * -inf. */
+ * -inf.  p is lens[s] - q_start[s + 1] + t as for the writing, also where that
+ * or lens[s] lies past the table, of which the positions below max_pages * page
+ * are seen; a token before the sequence (p < 0) sees none. */
 int bfp200_kv4_attention_dev(const bfp200_kv4_attention_args* args, void* stream);
 /* Bytes of workspace that the call needs: 0 without tokens or sequences, and
  * where max_pages * page is at most 128 (256 for HD <= 64) and the call is no

@@ -74,3 +74,47 @@ def test_attention_after_an_empty_call(n_seq):
     q = _rand(rng, (1, 3, 64), "float32")
     out, lse = kv4.attention(q, case.pool, case.q_start, case.len_t, case.bt, return_lse=True)
     _check_rows(q, *case.kv[0], _visible([699], 700, True, 0), out, lse, "float32")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 9), (False, 0), (False, 9)])
+@pytest.mark.parametrize("HD,group,new", FORMS)
+def test_attention_lengths_past_the_table(HD, group, new, causal, window, dtype):
+    """Tokens keep their positions lens - q_start[s + 1] + t where the table is
+    shorter than lens: they see what the table holds of them, as append places
+    them.  The sequences end 2 positions past the table, within the call's
+    tokens past it, and far past it."""
+    from bfp200 import kv4
+    rng = np.random.default_rng(HD + new)
+    cap = 64
+    over = [cap + 2, cap + new, cap, cap + 300, 2 ** 31 - 1]
+    case = Case(rng, [cap] * len(over), [new] * len(over), 2, HD, 16, extra_cols=0)
+    q = _rand(rng, (case.tokens, 2 * group, HD), dtype)
+    out, lse = kv4.attention(q, case.pool, case.q_start, _i32(over), case.bt, causal=causal, window=window, return_lse=True)
+    for s, L in enumerate(over):
+        rows = slice(s * new, (s + 1) * new)
+        see = _visible(L - new + np.arange(new), cap, causal, window)
+        _check_rows(q[rows], *case.kv[s], see, out[rows], lse[rows], dtype)
+
+
+@pytest.mark.parametrize("HD,group,new", FORMS)
+def test_append_and_attention_agree_past_the_table(HD, group, new):
+    """What append writes of a call that runs past its table, attention sees
+    under the mask of the positions that append gave the tokens."""
+    import torch
+    from bfp200 import kv4
+    rng = np.random.default_rng(3)
+    new, cap = new + 1, 16
+    L = cap + new - 1                                        # the first token still has a place
+    k, v, q = (_rand(rng, (new, h, HD), "bfloat16") for h in (1, 1, group))
+    pool = torch.full((1, 1, 16, HD * 9 // 8), 0xFF, dtype=torch.uint8, device="cuda")
+    args = (pool, _i32([0, new]), _i32([L]), _i32([[0]]))
+    kf, vf = (rng.standard_normal((cap, 1, HD)) for _ in range(2))
+    rec = pool.cpu().numpy()[0].reshape(1, -1).copy()
+    for p in range(cap):
+        O.put(rec[0], p, 16, kf[p, 0], vf[p, 0])
+    pool.copy_(torch.from_numpy(rec.reshape(tuple(pool.shape))))
+    kv4.append(pool, k, v, *args[1:])
+    kf[cap - 1], vf[cap - 1] = _f64(k)[0], _f64(v)[0]
+    out, lse = kv4.attention(q, *args, return_lse=True)
+    _check_rows(q, O.value(*O.quantize(kf)), O.value(*O.quantize(vf)), _visible(L - new + np.arange(new), cap, True, 0), out, lse, "bfloat16")

@@ -60,8 +60,8 @@ constexpr int MINB = 4;            // blocks that are not worth a second CTA: on
 // the cuts (256 sequences of up to 2047, 9 / 3 heads of 64: 41.7 us at 0, 36.2 at 4).
 constexpr int ITEM = 4;
 // ---- the split ---------------------------------------------------------------
-struct Seq {
-  int q0, n_q, len, blk0, nb, rt;  // first token, tokens, positions, first block, blocks plus ITEM, row tiles
+struct Seq : Span {
+  int blk0, nb, rt;                // first block, blocks plus ITEM, row tiles
 };
 
 // Blocks before each sequence (or chunk of `per` sequences, where there are
@@ -70,31 +70,25 @@ constexpr int SCH = 256;
 struct Sched {
   long long pre[SCH + 1];
   long long total, geff, delta;
-  int q0[SCH], n_q[SCH], len[SCH];   // the sequences themselves, where per == 1
+  Span span[SCH];                    // the sequences themselves, where per == 1
   long long wsum[16], wit[16];
   int per;
 };
 
-// What follows from a sequence's first token, tokens and length.
+// What follows from a sequence's tokens and positions.
 template <int NR, int BLK>
-__device__ __forceinline__ Seq seq_make(const AttnArgs& a, int q0, int n_q, int len) {
+__device__ __forceinline__ Seq seq_make(const AttnArgs& a, const Span& p) {
   Seq r;
-  r.q0 = q0;
-  r.n_q = n_q;
-  r.len = len;
-  const long long first = a.window ? (long long)len - n_q - a.window + 1 : 0;
-  r.blk0 = first > 0 ? min((int)(first / BLK), max(len - 1, 0) / BLK) : 0;
-  r.nb = max((len + BLK - 1) / BLK - r.blk0, 1) + ITEM;
-  const long long rows = (long long)n_q * a.group;
+  static_cast<Span&>(r) = p;
+  const long long first = a.window ? (long long)p.qp0 - a.window + 1 : 0;
+  r.blk0 = first > 0 ? min((int)(first / BLK), max(p.len - 1, 0) / BLK) : 0;
+  r.nb = max((p.len + BLK - 1) / BLK - r.blk0, 1) + ITEM;
+  const long long rows = (long long)p.n_q * a.group;
   r.rt = (int)((rows + NR - 1) / NR);
   return r;
 }
 template <int NR, int BLK>
-__device__ __forceinline__ Seq seq_of(const AttnArgs& a, int s) {
-  const int qs = min(max(__ldg(a.b.q_start + s), 0), a.b.T);
-  const int qe = min(max(__ldg(a.b.q_start + s + 1), qs), a.b.T);
-  return seq_make<NR, BLK>(a, qs, qe - qs, min(max(__ldg(a.b.lens + s), 0), a.b.max_pages << a.b.page_shift));
-}
+__device__ __forceinline__ Seq seq_of(const AttnArgs& a, int s) { return seq_make<NR, BLK>(a, span_of(a.b, s)); }
 
 // Fills the schedule; every thread of the CTA takes part.
 template <int NR, int BLK, int THR>
@@ -109,7 +103,7 @@ __device__ void make_sched(const AttnArgs& a, Sched& s) {
     if (c >= SCH) break;
     for (int i = c * per; i < min((c + 1) * per, a.b.n_seq); ++i) {
       const Seq q = seq_of<NR, BLK>(a, i);
-      if (per == 1) { s.q0[c] = q.q0; s.n_q[c] = q.n_q; s.len[c] = q.len; }
+      if (per == 1) s.span[c] = q;
       const long long n = (long long)q.rt * a.b.H;
       items += n;
       w[k] += n * q.nb;
@@ -167,7 +161,7 @@ __device__ Item item_at(const AttnArgs& a, const Sched& s, long long x) {
   long long at = s.pre[lo];
   if (s.per == 1) {
     it.seq = lo;
-    it.q = seq_make<NR, BLK>(a, s.q0[lo], s.n_q[lo], s.len[lo]);
+    it.q = seq_make<NR, BLK>(a, s.span[lo]);
   } else {
     it.seq = lo * s.per;
     #pragma unroll 1
@@ -276,7 +270,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::W * 32, Shape<HD, NT>::CTAS) at
     if (xe <= x) break;                                               // lengths changed during the call
     const int rt = it.q.rt, h = it.idx / rt, r0 = (it.idx - h * rt) * NR;
     const int rows = min(NR, it.q.n_q * a.group - r0);
-    const int len = it.q.len, qp0 = len - it.q.n_q;                   // position of the sequence's first query
+    const int len = it.q.len, qp0 = it.q.qp0;
     // ---- rows: queries to operand registers
     for (int i = tid; i < HD / 16 * NT * 32; i += W * 32) {
       const int l = i & 31, nt = (i >> 5) % NT, st = i / (32 * NT);

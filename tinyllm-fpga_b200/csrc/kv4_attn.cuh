@@ -41,6 +41,20 @@ struct AttnArgs {
   int grid;                        // CTAs of the first launch
 };
 
+// A sequence as the call describes it.  The last token before q_start[s + 1] is at
+// position lens[s] - 1, as for append and read: tokens keep their positions where
+// the table holds fewer than lens[s] (or the call fewer rows than q_start says).
+struct Span { int q0, n_q, len, qp0; };   // first token, tokens, positions that the table holds, position of the first token
+__device__ __forceinline__ Span span_of(const Batch& b, int s) {
+  const int end = __ldg(b.q_start + s + 1), len = max(__ldg(b.lens + s), 0);
+  Span r;
+  r.q0 = min(max(__ldg(b.q_start + s), 0), b.T);
+  r.n_q = min(max(end, r.q0), b.T) - r.q0;
+  r.len = min(len, b.max_pages << b.page_shift);
+  r.qp0 = len - (max(end, r.q0) - r.q0);
+  return r;
+}
+
 // ---- arithmetic ------------------------------------------------------------------
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const unsigned (&a)[4], uint2 b) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"

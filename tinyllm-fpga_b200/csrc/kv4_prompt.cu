@@ -115,24 +115,23 @@ constexpr int CH = 256;
 struct Plan {
   long long pre[CH + 1];                     // blocks before each sequence, or chunk of `per` sequences
   long long total, geff, delta;
-  int q0[CH], n_q[CH], len[CH];              // the sequences, where per == 1
+  Span span[CH];                             // the sequences, where per == 1
   long long items;
   int per;
 };
-struct PSeq { int q0, n_q, len, rt, seq; };
+struct PSeq : Span { int rt, seq; };         // row tiles, index
 struct Tiles { int first, nb; };             // first block of a row tile, its blocks plus ITEM
 
-__device__ __forceinline__ PSeq seq_at(const AttnArgs& a, int s) {
+__device__ __forceinline__ PSeq seq_make(const AttnArgs& a, int s, const Span& p) {
   PSeq r;
+  static_cast<Span&>(r) = p;
   r.seq = s;
-  r.q0 = min(max(__ldg(a.b.q_start + s), 0), a.b.T);
-  r.n_q = min(max(__ldg(a.b.q_start + s + 1), r.q0), a.b.T) - r.q0;
-  r.len = min(max(__ldg(a.b.lens + s), 0), a.b.max_pages << a.b.page_shift);
-  r.rt = (int)(((long long)r.n_q * a.group + PR - 1) / PR);
+  r.rt = (int)(((long long)p.n_q * a.group + PR - 1) / PR);
   return r;
 }
+__device__ __forceinline__ PSeq seq_at(const AttnArgs& a, int s) { return seq_make(a, s, span_of(a.b, s)); }
 __device__ __forceinline__ Tiles tiles_of(const AttnArgs& a, const PSeq& q, int rt) {
-  const int qp0 = q.len - q.n_q;
+  const int qp0 = q.qp0;
   const int j0 = (int)((long long)rt * PR / a.group), j1 = (int)min((long long)q.n_q - 1, ((long long)rt * PR + PR - 1) / a.group);
   const int hi = qp0 + j1 < 0 ? 0 : a.causal ? min(q.len, qp0 + j1 + 1) : q.len;
   const long long lo = a.window ? max(0LL, (long long)qp0 + j0 - a.window + 1) : 0;
@@ -160,7 +159,7 @@ __device__ __forceinline__ void make_plan(const AttnArgs& a, Plan& s) {
     long long w = 0, items = 0;
     for (int i = c * per; i < min((c + 1) * per, a.b.n_seq); ++i) {
       const PSeq q = seq_at(a, i);
-      if (per == 1) { s.q0[c] = q.q0; s.n_q[c] = q.n_q; s.len[c] = q.len; }
+      if (per == 1) s.span[c] = q;
       long long n = 0;
       if (wide) n = head_blocks(a, q);
       else for (int r = 0; r < q.rt; ++r) n += tiles_of(a, q, r).nb;
@@ -224,11 +223,7 @@ __device__ __forceinline__ PItem item_of(const AttnArgs& a, const Plan& s, long 
   PItem it;
   long long at = s.pre[lo], w1;
   if (s.per == 1) {
-    it.q.seq = lo;
-    it.q.q0 = s.q0[lo];
-    it.q.n_q = s.n_q[lo];
-    it.q.len = s.len[lo];
-    it.q.rt = (int)(((long long)it.q.n_q * a.group + PR - 1) / PR);
+    it.q = seq_make(a, lo, s.span[lo]);
     w1 = div_small(s.pre[lo + 1] - at, a.b.H);
   } else {
     for (int i = lo * s.per;; ++i) {
@@ -418,11 +413,11 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
   };
   // what a row of the segment sees: positions lo .. hi - 1
   const auto hi_at = [&](const Seg& g, int j) {
-    const int p = g.it.q.len - g.it.q.n_q + j;
+    const int p = g.it.q.qp0 + j;
     return p < 0 ? 0 : a.causal ? min(g.it.q.len, p + 1) : g.it.q.len;
   };
   const auto lo_at = [&](const Seg& g, int j) {
-    return a.window ? (int)max(0LL, (long long)g.it.q.len - g.it.q.n_q + j - a.window + 1) : 0;
+    return a.window ? (int)max(0LL, (long long)g.it.q.qp0 + j - a.window + 1) : 0;
   };
 
   if (warp < 8) {
