@@ -391,7 +391,7 @@ typedef struct bfp200_kv4_attention_args {
  * (causal) and k > p - window (window > 0); one that sees none gives zeros and
  * -inf.  p is lens[s] - q_start[s + 1] + t as for the writing, also where that
  * or lens[s] lies past the table, of which the positions below max_pages * page
- * are seen; a token before the sequence (p < 0) sees none. */
+ * are seen; a token before the sequence (p < 0) or outside q_start sees none. */
 int bfp200_kv4_attention_dev(const bfp200_kv4_attention_args* args, void* stream);
 /* Bytes of workspace that the call needs: 0 without tokens or sequences, and
  * where max_pages * page is at most 128 (256 for HD <= 64) and the call is no

@@ -118,3 +118,33 @@ def test_append_and_attention_agree_past_the_table(HD, group, new):
     kf[cap - 1], vf[cap - 1] = _f64(k)[0], _f64(v)[0]
     out, lse = kv4.attention(q, *args, return_lse=True)
     _check_rows(q, O.value(*O.quantize(kf)), O.value(*O.quantize(vf)), _visible(L - new + np.arange(new), cap, True, 0), out, lse, "bfloat16")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("HD,group,new", FORMS)
+def test_attention_rows_of_no_sequence(HD, group, new, dtype):
+    """Rows before q_start[0] and from q_start[n_seq] on give zeros and
+    -infinity, in outputs with any strides, and change nothing elsewhere."""
+    import torch
+    from bfp200 import kv4
+    rng = np.random.default_rng(HD * new)
+    n, lead, tail = 3, 5, 70
+    case = Case(rng, [100] * n, [new] * n, 2, HD, 32)
+    T, HQ = lead + n * new + tail, 2 * group
+    q = _rand(rng, (T, HQ, HD), dtype)
+    qs = case.q_start + lead
+    wide = torch.full((T, HQ + 2, HD), float("nan"), dtype=_dt(dtype), device="cuda")
+    with _empty_is_nan():
+        for out in (None, wide[:, 1:-1]):
+            got, lse = kv4.attention(q, case.pool, qs, case.len_t, case.bt, out=out, return_lse=True)
+            for s in range(n):
+                rows = slice(lead + s * new, lead + (s + 1) * new)
+                _check_rows(q[rows], *case.kv[s], _visible(100 - new + np.arange(new), 100, True, 0), got[rows], lse[rows], dtype)
+            for rows in (slice(0, lead), slice(lead + n * new, T)):
+                assert (got[rows] == 0).all() and (lse[rows] == -torch.inf).all()
+        assert wide[:, 0].isnan().all() and wide[:, -1].isnan().all()
+        # every row of no sequence: sequences without tokens
+        got, lse = kv4.attention(q, case.pool, _i32([T] * (n + 1)), case.len_t, case.bt, return_lse=True)
+        assert (got == 0).all() and (lse == -torch.inf).all()
+        got, lse = kv4.attention(q, case.pool, _i32([0] * (n + 1)), case.len_t, case.bt, return_lse=True)
+        assert (got == 0).all() and (lse == -torch.inf).all()

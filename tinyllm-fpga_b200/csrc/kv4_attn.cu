@@ -255,6 +255,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::W * 32, Shape<HD, NT>::CTAS) at
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   make_sched<NR, BLK, W * 32>(a, sch);
+  clear_rows<T, HD>(a, blockIdx.x * W + warp, gridDim.x * W);
   if (tid == 0 && a.cuts) a.cuts[blockIdx.x].parts = 0;
   if ((long long)blockIdx.x >= sch.geff || sch.total == 0) return;
   long long x = bound<NR, BLK>(a, sch, (long long)blockIdx.x + (lane & 1));   // both bounds at once

@@ -55,6 +55,23 @@ __device__ __forceinline__ Span span_of(const Batch& b, int s) {
   return r;
 }
 
+// Rows of no sequence, before q_start[0] and from q_start[n_seq] on: zeros and
+// -infinity, a row a warp.  Where every row belongs to a sequence it costs two
+// loads.
+template <typename T, int HD>
+__device__ __forceinline__ void clear_rows(const AttnArgs& a, int warp, int warps) {
+  const int lead = a.b.n_seq ? min(max(__ldg(a.b.q_start), 0), a.b.T) : 0;
+  const int tail = a.b.n_seq ? min(max(__ldg(a.b.q_start + a.b.n_seq), lead), a.b.T) : 0;
+  #pragma unroll 1
+  for (int t = warp < lead ? warp : tail + warp - lead; t < a.b.T; t = t + warps < lead || t >= tail ? t + warps : t + warps - lead + tail) {
+    #pragma unroll 1
+    for (int i = threadIdx.x & 31; i < a.HQ * HD; i += 32)
+      static_cast<T*>(a.out)[t * a.o_ts + i / HD * a.o_hs + i % HD] = from_f<T>(0.f);
+    if (a.lse)
+      for (int i = threadIdx.x & 31; i < a.HQ; i += 32) a.lse[(long long)t * a.HQ + i] = -INFINITY;
+  }
+}
+
 // ---- arithmetic ------------------------------------------------------------------
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const unsigned (&a)[4], uint2 b) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"

@@ -44,7 +44,7 @@ constexpr int MIN_SHARE = 8;                 // blocks that are not worth a seco
 // An item's queries, first block and outputs, in blocks (8192 tokens, 32 / 8
 // heads of 128: 730 us at 3, 646 at 6, 666 at 9).
 constexpr int ITEM = 6;
-constexpr int THREADS = 512;                  // softmax 2 x 4 warps, decoding 4, MMA 2 (and 2 that wait at the end)
+constexpr int THREADS = 512;                  // softmax 2 x 4 warps, decoding 4, MMA 2, rows of no sequence 2
 constexpr int SPIN = 1 << 20;
 
 __device__ __forceinline__ void mb_init(unsigned long long* bar, unsigned count) {
@@ -732,6 +732,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
         __syncwarp();
       }
     });
+    else clear_rows<T, HD>(a, blockIdx.x * 2 + warp - 14, gridDim.x * 2);
   }
   __syncwarp();
   if (warp == 12 || warp == 13) {                           // every MMA has ended before the tensor memory goes back
