@@ -364,7 +364,9 @@ typedef struct bfp200_kv4_append_args {
   long long H_Q, n_pos, rot, dtype, interleaved;   /* H_Q 0: no queries */
 } bfp200_kv4_append_args;
 /* Rotates the call's keys and queries, quantizes keys and values and writes
- * them to their pages. */
+ * them to their pages.  Queries of tokens without a position are rotated too,
+ * without positions_dev by their place beside the nearest sequence (by 0 where
+ * the call has none), held to the table. */
 int bfp200_kv4_append_dev(const bfp200_kv4_append_args* args, void* stream);
 
 typedef struct bfp200_kv4_read_args {

@@ -148,3 +148,35 @@ def test_attention_rows_of_no_sequence(HD, group, new, dtype):
         assert (got == 0).all() and (lse == -torch.inf).all()
         got, lse = kv4.attention(q, case.pool, _i32([0] * (n + 1)), case.len_t, case.bt, return_lse=True)
         assert (got == 0).all() and (lse == -torch.inf).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [0, 40])
+@pytest.mark.parametrize("T", [1, 300])
+def test_calls_without_sequences(T, cols, dtype):
+    """Tokens of no sequence at all: zeros from read and attention, nothing
+    written by append, whose queries are turned by their `positions`, without
+    them by position 0."""
+    import torch
+    from bfp200 import kv4
+    rng = np.random.default_rng(T)
+    pool = torch.full((2, 2, 16, 72), 0x5A, dtype=torch.uint8, device="cuda")
+    before = pool.clone()
+    b = (_i32([0]), _i32([]), torch.zeros((0, cols), dtype=torch.int32, device="cuda"))
+    k, v, q = (_rand(rng, (T, h, 64), dtype) for h in (2, 2, 6))
+    table = kv4.rope_table(640, 64)
+    pos = rng.integers(0, 640, T)
+    cs = table.cpu().numpy()
+    with _empty_is_nan():
+        for rd in DTYPES:
+            rk, rv = kv4.read(pool, *b, T, dtype=_dt(rd))
+            assert (rk == 0).all() and (rv == 0).all()
+        out, lse = kv4.attention(q, pool, *b, return_lse=True)
+        assert (out == 0).all() and (lse == -torch.inf).all()
+        assert torch.equal(kv4.append(pool, k, v, *b, q=q), q)
+        got = kv4.append(pool, k, v, *b, q=q, table=table)
+        assert np.array_equal(_f64(got), _rounded(O.rotate32(_f32(q), cs[np.zeros(T, int)], 64, False), dtype))
+        got = kv4.append(pool, k, v, *b, q=q, table=table, positions=_i32(pos))
+        assert np.array_equal(_f64(got), _rounded(O.rotate32(_f32(q), cs[pos], 64, False), dtype))
+        assert kv4.append(pool, k, v, *b) is None
+    assert torch.equal(pool, before)

@@ -291,10 +291,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) append_kernel(con
     }
   };
   load(grp * a.group_passes);
-  const int seq = seq_of_token(a.b, t);
-  const int q_end = __ldg(a.b.q_start + seq + 1);
-  const int pos = __ldg(a.b.lens + seq) - q_end + t;
-  const bool held = t >= __ldg(a.b.q_start + seq) && t < q_end && pos >= 0 && (pos >> a.b.page_shift) < a.b.max_pages;
+  int seq = 0, q_end = 0, pos = -1;
+  bool held = false;
+  if (a.b.n_seq) {
+    seq = seq_of_token(a.b, t);
+    q_end = __ldg(a.b.q_start + seq + 1);
+    pos = __ldg(a.b.lens + seq) - q_end + t;
+    held = t >= __ldg(a.b.q_start + seq) && t < q_end && pos >= 0 && (pos >> a.b.page_shift) < a.b.max_pages;
+  }
   const int pg = held ? __ldg(a.b.bt + (long long)seq * a.b.bt_ld + (pos >> a.b.page_shift)) : -1;
   const bool store = held && (unsigned)pg < (unsigned)a.b.n_pages;
   const int rot = a.r.table ? a.r.rot : 0, half = rot >> 1;
@@ -627,7 +631,7 @@ extern "C" int bfp200_kv4_append_dev(const bfp200_kv4_append_args* in, void* str
       return bad("the rotation table is shorter than max_pages * page positions");
     if (reinterpret_cast<uintptr_t>(r.table_dev) & 7u) return bad("the table must be 8-byte aligned");
   }
-  if (a.b.T == 0 || a.b.n_seq == 0) return BFP200_OK;
+  if (a.b.T == 0 || (a.b.n_seq == 0 && r.H_Q == 0)) return BFP200_OK;
   if (!r.k_dev || !r.v_dev || (r.H_Q > 0 && (!r.q_dev || !r.q_out_dev))) return bad("null pointer");
   const uintptr_t all = reinterpret_cast<uintptr_t>(r.k_dev) | reinterpret_cast<uintptr_t>(r.v_dev) |
                         (r.H_Q ? reinterpret_cast<uintptr_t>(r.q_dev) | reinterpret_cast<uintptr_t>(r.q_out_dev) : 0);
@@ -663,7 +667,7 @@ extern "C" int bfp200_kv4_read_dev(const bfp200_kv4_read_args* in, void* stream)
   ReadArgs a;
   if (int rc = fill_batch(in->batch, &a.b, who)) return rc;
   if (!elem_size(in->dtype)) return bad("dtype must be BFP200_F32, BFP200_F16 or BFP200_BF16");
-  if (a.b.T == 0 || a.b.n_seq == 0) return BFP200_OK;
+  if (a.b.T == 0) return BFP200_OK;
   if (!in->k_out_dev || !in->v_out_dev) return bad("null pointer");
   if ((reinterpret_cast<uintptr_t>(in->k_out_dev) | reinterpret_cast<uintptr_t>(in->v_out_dev)) & 15u)
     return bad("outputs must be 16-byte aligned");
@@ -672,6 +676,12 @@ extern "C" int bfp200_kv4_read_dev(const bfp200_kv4_read_args* in, void* stream)
   a.k = in->k_out_dev; a.v = in->v_out_dev;
   a.span = 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a.b.n_seq == 0) {                                     // tokens of no sequence
+    const size_t bytes = (size_t)a.b.T * a.b.H * (size_t)in->batch.HD * elem_size(in->dtype);
+    cudaError_t z = cudaMemsetAsync(a.k, 0, bytes, s);
+    if (z == cudaSuccess) z = cudaMemsetAsync(a.v, 0, bytes, s);
+    return z == cudaSuccess ? BFP200_OK : cuda_fail(who, z);
+  }
   const cudaError_t e = by_hd((int)in->batch.HD, [&](auto hd) {
     constexpr int N = decltype(hd)::value;
     return in->dtype == BFP200_F32 ? launch_read<float, N>(a, s)

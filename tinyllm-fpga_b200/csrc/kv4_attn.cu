@@ -681,7 +681,7 @@ cudaError_t launch_attn(AttnArgs a, int n_sm, float* ws, cudaStream_t s) {
   cudaError_t e = allow_smem(kern, smem, allowed);
   if (e != cudaSuccess) return e;
   a.grid = n_sm * SH::CTAS;
-  const bool whole = never_cut<HD>(a.b);
+  const bool whole = a.b.n_seq == 0 || never_cut<HD>(a.b);
   a.cuts = whole ? nullptr : reinterpret_cast<Cut*>(ws);
   a.part = whole ? nullptr : reinterpret_cast<float*>(a.cuts + a.grid);
   kern<<<a.grid, W * 32, smem, s>>>(a);
@@ -698,11 +698,13 @@ cudaError_t launch_attn(AttnArgs a, int n_sm, float* ws, cudaStream_t s) {
 // from some 300 (100 tokens of 9 / 3 heads: 90 against 96; 48 tokens: 66 against 57).
 // 32-bit queries would not fit its shared memory.
 int pick_nt(const Batch& b, int group, int hd, bool wide) {
+  if (b.n_seq == 0) return 1;
   const long long rows = ((long long)b.T + b.n_seq - 1) / b.n_seq * group;
   return rows <= 8 ? 1 : rows <= 16 ? 2 : wide || rows <= (hd > 64 ? 32 : 256) ? 4 : 8;
 }
 // Room for the partial sums of any call with this head dim; none where nothing is cut.
 size_t ws_bytes(const Batch& b, int hd, int nt, int n_sm) {
+  if (b.n_seq == 0) return 0;
   if (nt != 8 && (hd > 64 ? never_cut<128>(b) : never_cut<64>(b))) return 0;
   size_t most = 0;
   for (int nt = 1; nt <= 4; nt *= 2) {
@@ -745,7 +747,7 @@ extern "C" int bfp200_kv4_attention_workspace(const bfp200_kv4_attention_args* i
   int n_sm = 0;
   if (int rc = device_ready(who, &n_sm)) return rc;
   const int hd = (int)in->batch.HD;
-  *bytes = b.T == 0 || b.n_seq == 0 ? 0 : ws_bytes(b, hd, pick_nt(b, (int)in->H_Q / b.H, hd, in->dtype == BFP200_F32), n_sm);
+  *bytes = b.T == 0 ? 0 : ws_bytes(b, hd, pick_nt(b, (int)in->H_Q / b.H, hd, in->dtype == BFP200_F32), n_sm);
   return BFP200_OK;
 }
 
@@ -761,7 +763,7 @@ extern "C" int bfp200_kv4_attention_dev(const bfp200_kv4_attention_args* in, voi
   if (r.H_Q < 1 || r.H_Q > (1LL << 16) || r.H_Q % a.b.H) return bad("H_Q must be a positive multiple of H_KV");
   if (r.window < 0) return bad("window must not be negative");
   if (!(r.scale - r.scale == 0.0)) return bad("scale must be finite");
-  if (a.b.T == 0 || a.b.n_seq == 0) return BFP200_OK;
+  if (a.b.T == 0) return BFP200_OK;
   if (!r.q_dev || !r.out_dev) return bad("null pointer");
   if ((reinterpret_cast<uintptr_t>(r.q_dev) | reinterpret_cast<uintptr_t>(r.out_dev)) % es ||
       reinterpret_cast<uintptr_t>(r.lse_dev) % 4 || reinterpret_cast<uintptr_t>(r.workspace_dev) % 16)
