@@ -399,6 +399,14 @@ int bfp200_kv4_attention_dev(const bfp200_kv4_attention_args* args, void* stream
  * where max_pages * page is at most 128 (256 for HD <= 64) and the call is no
  * prompt; else the same for every call of a head dim (some 40 MB at most). */
 int bfp200_kv4_attention_workspace(const bfp200_kv4_attention_args* args, size_t* bytes);
+/* Waits for `stream` and says how the last call with this workspace ended:
+ * BFP200_ETIMEOUT if a bounded wait of its kernel ran out (the rows that it
+ * left undone are NaN, in out_dev and lse_dev), else BFP200_OK.  Only prompts
+ * have such waits.  NULL, of a call that needs no workspace, is BFP200_OK. */
+int bfp200_kv4_attention_status(const void* workspace_dev, void* stream);
+/* Self-test of the above: a call of the prompts' kernel (16-bit, enough rows a
+ * sequence; EINVAL otherwise) whose waits all run out at once. */
+int bfp200_kv4_wait_probe(const bfp200_kv4_attention_args* args, void* stream);
 
 /* Stage dump layout of bfp200_fwd_layer (mirrors the N1..D dumps of
  * gen_smollm_blockfp_bfp.py:393-426): n1 q k v attn o h1 n2 g u mlp d, where

@@ -180,3 +180,69 @@ def test_calls_without_sequences(T, cols, dtype):
         assert np.array_equal(_f64(got), _rounded(O.rotate32(_f32(q), cs[pos], 64, False), dtype))
         assert kv4.append(pool, k, v, *b) is None
     assert torch.equal(pool, before)
+
+
+def _raw_attention(fn, case, q, out, lse, ws):
+    """A C entry point that takes bfp200_kv4_attention_args, causal, on the default stream."""
+    import torch
+    from bfp200 import _lib, kv4
+    args = kv4._ATTENTION.pack(*kv4._batch(case.pool, case.q_start, case.len_t, case.bt, q.shape[0])[1], q.data_ptr(), out.data_ptr(),
+                               lse.data_ptr(), ws.data_ptr(), ws.numel(), *q.stride()[:2], *out.stride()[:2], q.shape[1],
+                               kv4._DTYPES[q.dtype], 1, 0, q.shape[2] ** -0.5)
+    return getattr(_lib.lib(), fn)(args, torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("HD,lens,new", [(128, [90, 50], 30), (64, [3000], 300), (128, [2000] * 40, 64)])
+def test_a_wait_that_runs_out_is_reported_to_its_caller(HD, lens, new, dtype):
+    """Whole items, one item cut over many CTAs, and more items than CTAs: every
+    row is NaN, the status says so, rows of no sequence keep their zeros, the
+    next call with the same workspace is right, and a Decoder hears nothing of
+    it."""
+    import torch
+    from bfp200 import BfpConfig, Decoder, _lib, kv4, synth
+    rng = np.random.default_rng(HD)
+    H, group, lead = 2, 8, 3
+    case = Case(rng, lens[:1], [new], H, HD, 64)              # (one filled sequence, read by all)
+    case.bt, case.len_t = case.bt.expand(len(lens), -1), _i32(lens)
+    case.q_start = _i32(lead + new * np.arange(len(lens) + 1))
+    T = lead + new * len(lens)
+    q = _rand(rng, (T, H * group, HD), dtype)
+    want, wl = kv4.attention(q, case.pool, case.q_start, case.len_t, case.bt, return_lse=True, check_done=True)
+    assert not want.isnan().any()
+    ws = torch.full((64 << 20,), 0xFF, dtype=torch.uint8, device="cuda")
+    status = lambda: _lib.lib().bfp200_kv4_attention_status(ws.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    for _ in range(2):
+        out, lse = torch.zeros_like(q), torch.zeros((T, H * group), device="cuda")
+        assert _raw_attention("bfp200_kv4_wait_probe", case, q, out, lse, ws) == _lib.OK
+        assert status() == _lib.ETIMEOUT and "timed out" in _lib.last_error()
+        assert out[lead:].isnan().all() and lse[lead:].isnan().all()
+        assert (out[:lead] == 0).all() and (lse[:lead] == -torch.inf).all()
+        assert _raw_attention("bfp200_kv4_attention_dev", case, q, out, lse, ws) == _lib.OK
+        assert status() == _lib.OK
+        assert torch.equal(out, want) and torch.equal(lse, wl)
+    assert _raw_attention("bfp200_kv4_wait_probe", case, q, out, lse, ws) == _lib.OK
+    cfg = BfpConfig(D=64, H_Q=1, H_KV=1, HD=64, FFN=128, NL=2, VOCAB=64, MAX_CTX=16, max_seqs=1)
+    with Decoder(cfg) as dec:
+        dec.load_image(synth.synthetic_image(cfg, 5))
+        assert len(dec.generate([[1, 2, 3]], 2)[0]) == 5
+    assert status() == _lib.ETIMEOUT
+
+
+def test_the_status_of_calls_without_waits():
+    import torch
+    from bfp200 import _lib, kv4
+    rng = np.random.default_rng(1)
+    L, stream = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    assert L.bfp200_kv4_attention_status(None, stream) == _lib.OK
+    assert L.bfp200_kv4_attention_status(4, stream) == _lib.EINVAL
+    case = Case(rng, [700], [1], 1, 64, 16)
+    ws = torch.full((64 << 20,), 0xFF, dtype=torch.uint8, device="cuda")
+    for dtype in DTYPES:
+        q = _rand(rng, (1, 3, 64), dtype)
+        out, lse = torch.zeros_like(q), torch.zeros((1, 3), device="cuda")
+        assert _raw_attention("bfp200_kv4_wait_probe", case, q, out, lse, ws) == _lib.EINVAL
+        ws.fill_(0xFF)
+        assert _raw_attention("bfp200_kv4_attention_dev", case, q, out, lse, ws) == _lib.OK
+        assert L.bfp200_kv4_attention_status(ws.data_ptr(), stream) == _lib.OK
+        kv4.attention(q, case.pool, case.q_start, case.len_t, case.bt, check_done=True)

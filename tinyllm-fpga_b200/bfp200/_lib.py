@@ -82,6 +82,8 @@ SIGNATURES = {
     "bfp200_kv4_read_dev": [_P, _P],
     "bfp200_kv4_attention_dev": [_P, _P],
     "bfp200_kv4_attention_workspace": [_P, C.POINTER(_Z)],
+    "bfp200_kv4_attention_status": [_P, _P],
+    "bfp200_kv4_wait_probe": [_P, _P],
 }
 NCCL_ID_BYTES = 128
 

@@ -113,13 +113,13 @@ _current_device = getattr(torch._C, "_cuda_getDevice", None) or (lambda: torch.c
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
-def _run(fn, packed, index):
+def _run(fn, arg, index):
     """Calls a C entry point on torch's current stream of GPU `index`."""
     if _current_device() == index:
-        rc = fn(packed, _raw_stream(index))
+        rc = fn(arg, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(packed, _raw_stream(index))
+            rc = fn(arg, _raw_stream(index))
     if rc:
         check(rc)
 
@@ -264,14 +264,18 @@ def read(pool, q_start, lens, block_table, tokens, dtype=torch.bfloat16):
     return k, v
 
 
-def attention(q, pool, q_start, lens, block_table, scale=None, causal=True, window=0, out=None, return_lse=False):
+def attention(q, pool, q_start, lens, block_table, scale=None, causal=True, window=0, out=None, return_lse=False,
+              check_done=False):
     """Softmax attention of q [tokens, H_Q, HD] over the cached positions of
     the tokens' sequences; H_Q a multiple of H_KV, query head i reads KV head
     i // (H_Q / H_KV).  A token at position p sees the positions k < lens[s]
     with k <= p (causal) and k > p - window (window > 0).  scale defaults to
     HD^-1/2.  Returns out, and with return_lse the log-sum-exp of the scaled
     scores (float32 [tokens, H_Q]) to join it with attention over other keys;
-    a token that sees nothing gets zeros and -inf."""
+    a token that sees nothing gets zeros and -inf.
+
+    The kernel of prompts has bounded waits; rows that one leaves undone are
+    NaN.  check_done waits for the call and raises BfpError (ETIMEOUT) then."""
     dev, code, t, hq, d, qt, qh = _acts(q, "q")
     where, b = _batch(pool, q_start, lens, block_table, t)
     if where != dev or b[7] != d:
@@ -292,4 +296,6 @@ def attention(q, pool, q_start, lens, block_table, scale=None, causal=True, wind
     _run(_fn("bfp200_kv4_attention_dev"),
          _ATTENTION.pack(*b, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, ws.data_ptr() if need else 0, need, qt, qh, ot, oh,
                          hq, code, causal, window, d ** -0.5 if scale is None else scale), dev)
+    if check_done and need:
+        _run(_fn("bfp200_kv4_attention_status"), ws.data_ptr(), dev)
     return (out, lse) if return_lse else out

@@ -57,7 +57,7 @@ class PagedDecoder:
             n1 = ops.rmsnorm_fp(h, self.g1[i], cfg.eps)
             q, k, v = (self._gpu(self._matvec(n1, lw[w]), n) for w, n in (("Wq", cfg.H_Q), ("Wk", cfg.H_KV), ("Wv", cfg.H_KV)))
             q = kv4.append(self.pools[i], k, v, q_start, lens, block_table, q=q, table=self.table)
-            attn = kv4.attention(q, self.pools[i], q_start, lens, block_table)
+            attn = kv4.attention(q, self.pools[i], q_start, lens, block_table, check_done=True)
             h = self._grid(h + self._matvec(attn.view(len(h), -1).double().cpu().numpy(), lw["Wo"]))
             n2 = ops.rmsnorm_fp(h, self.g2[i], cfg.eps)
             mlp = ops.silu_fp(self._matvec(n2, lw["Wg"])) * self._matvec(n2, lw["Wu"])

@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::W * 32, Shape<HD, NT>::CTAS) at
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   make_sched<NR, BLK, W * 32>(a, sch);
   clear_rows<T, HD>(a, blockIdx.x * W + warp, gridDim.x * W);
-  if (tid == 0 && a.cuts) a.cuts[blockIdx.x].parts = 0;
+  if (tid == 0 && a.cuts) a.cuts[blockIdx.x] = Cut{};
   if ((long long)blockIdx.x >= sch.geff || sch.total == 0) return;
   long long x = bound<NR, BLK>(a, sch, (long long)blockIdx.x + (lane & 1));   // both bounds at once
   const long long x1 = __shfl_sync(0xffffffffu, x, 1);
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::W * 32, Shape<HD, NT>::CTAS) at
       const long long c = blockIdx.x;
       long long e = min(sch.geff, div_small(it.end * sch.geff + sch.total - 1, sch.total));
       while (e - 1 > c + 1 && bound<NR, BLK>(a, sch, e - 1) >= it.end) --e;
-      a.cuts[c] = Cut{(int)(e - c), it.q.q0, rows, r0, h * a.group, {0, 0, 0}};
+      a.cuts[c] = Cut{(int)(e - c), it.q.q0, rows, r0, h * a.group, 0, {0, 0}};
     }
     float* part = a.part + ((long long)blockIdx.x * 2 + (x > it.start ? 0 : 1)) * NR * (HD + 2);
     for (int i = tid; i < rows * (HD / 4); i += W * 32) {
@@ -671,7 +671,7 @@ template <int HD> bool never_cut(const Batch& b) { return (long long)b.max_pages
 static_assert(MINB + ITEM <= 2 * (ITEM + 1), "items of MINB blocks stay whole");
 
 template <typename T, int HD, int NT>
-cudaError_t launch_attn(AttnArgs a, int n_sm, float* ws, cudaStream_t s) {
+cudaError_t launch_attn(AttnArgs a, int n_sm, void* ws, cudaStream_t s) {
   using SH = Shape<HD, NT>;
   constexpr int W = SH::W, NR = NT * 8;
   constexpr size_t smem = SH::template smem<Kind<T>::QS>();
@@ -682,7 +682,8 @@ cudaError_t launch_attn(AttnArgs a, int n_sm, float* ws, cudaStream_t s) {
   if (e != cudaSuccess) return e;
   a.grid = n_sm * SH::CTAS;
   const bool whole = a.b.n_seq == 0 || never_cut<HD>(a.b);
-  a.cuts = whole ? nullptr : reinterpret_cast<Cut*>(ws);
+  a.status = whole ? nullptr : static_cast<Status*>(ws);
+  a.cuts = whole ? nullptr : reinterpret_cast<Cut*>(a.status + 1);
   a.part = whole ? nullptr : reinterpret_cast<float*>(a.cuts + a.grid);
   kern<<<a.grid, W * 32, smem, s>>>(a);
   e = cudaGetLastError();
@@ -708,7 +709,7 @@ size_t ws_bytes(const Batch& b, int hd, int nt, int n_sm) {
   if (nt != 8 && (hd > 64 ? never_cut<128>(b) : never_cut<64>(b))) return 0;
   size_t most = 0;
   for (int nt = 1; nt <= 4; nt *= 2) {
-    const size_t grid = (size_t)n_sm * 4, b = grid * (sizeof(Cut) + 2 * nt * 8 * (hd + 2) * 4);
+    const size_t grid = (size_t)n_sm * 4, b = sizeof(Status) + grid * (sizeof(Cut) + 2 * nt * 8 * (hd + 2) * 4);
     most = b > most ? b : most;
   }
   const size_t p = prompt_ws_bytes(hd, n_sm);
@@ -716,43 +717,23 @@ size_t ws_bytes(const Batch& b, int hd, int nt, int n_sm) {
 }
 
 template <typename T, int HD>
-cudaError_t by_nt(const AttnArgs& a, int nt, int n_sm, float* ws, cudaStream_t s) {
+cudaError_t by_nt(const AttnArgs& a, int nt, int n_sm, int spin, void* ws, cudaStream_t s) {
   if constexpr (!std::is_same<T, float>::value)
-    if (nt == 8) return launch_prompt<T, HD>(a, n_sm, ws, s);
+    if (nt == 8) return launch_prompt<T, HD>(a, n_sm, spin, ws, s);
   return nt == 1 ? launch_attn<T, HD, 1>(a, n_sm, ws, s)
        : nt == 2 ? launch_attn<T, HD, 2>(a, n_sm, ws, s)
                  : launch_attn<T, HD, 4>(a, n_sm, ws, s);
 }
 template <typename T>
-cudaError_t by_hd(int hd, const AttnArgs& a, int nt, int n_sm, float* ws, cudaStream_t s) {
-  return hd == 32 ? by_nt<T, 32>(a, nt, n_sm, ws, s)
-       : hd == 64 ? by_nt<T, 64>(a, nt, n_sm, ws, s)
-       : hd == 96 ? by_nt<T, 96>(a, nt, n_sm, ws, s)
-                  : by_nt<T, 128>(a, nt, n_sm, ws, s);
+cudaError_t by_hd(int hd, const AttnArgs& a, int nt, int n_sm, int spin, void* ws, cudaStream_t s) {
+  return hd == 32 ? by_nt<T, 32>(a, nt, n_sm, spin, ws, s)
+       : hd == 64 ? by_nt<T, 64>(a, nt, n_sm, spin, ws, s)
+       : hd == 96 ? by_nt<T, 96>(a, nt, n_sm, spin, ws, s)
+                  : by_nt<T, 128>(a, nt, n_sm, spin, ws, s);
 }
 
-}  // namespace
-}  // namespace kv4
-}  // namespace bfp
-
-using namespace bfp::kv4;
-
-extern "C" int bfp200_kv4_attention_workspace(const bfp200_kv4_attention_args* in, size_t* bytes) {
-  const char* who = "kv4_attention_workspace";
-  const auto bad = [&](const char* what) { return bfp200_set_error(BFP200_EINVAL, std::string(who) + ": " + what); };
-  if (!in || !bytes) return bad("no arguments");
-  Batch b;
-  if (int rc = fill_batch(in->batch, &b, who)) return rc;
-  if (in->H_Q < 1 || in->H_Q % b.H) return bad("H_Q must be a positive multiple of H_KV");
-  int n_sm = 0;
-  if (int rc = device_ready(who, &n_sm)) return rc;
-  const int hd = (int)in->batch.HD;
-  *bytes = b.T == 0 ? 0 : ws_bytes(b, hd, pick_nt(b, (int)in->H_Q / b.H, hd, in->dtype == BFP200_F32), n_sm);
-  return BFP200_OK;
-}
-
-extern "C" int bfp200_kv4_attention_dev(const bfp200_kv4_attention_args* in, void* stream) try {
-  const char* who = "kv4_attention_dev";
+// probe: a call of the prompts' kernel, whose waits give up at once
+int attention(const char* who, const bfp200_kv4_attention_args* in, bool probe, void* stream) {
   const auto bad = [&](const char* what) { return bfp200_set_error(BFP200_EINVAL, std::string(who) + ": " + what); };
   if (!in) return bad("no arguments");
   const bfp200_kv4_attention_args& r = *in;
@@ -785,16 +766,62 @@ extern "C" int bfp200_kv4_attention_dev(const bfp200_kv4_attention_args* in, voi
   a.grid = 0;
   a.part = nullptr;
   const int hd = (int)r.batch.HD, nt = pick_nt(a.b, a.group, hd, r.dtype == BFP200_F32);
+  if (probe && nt != 8) return bad("not a call of the prompts' kernel");
+  const int spin = probe ? 0 : SPIN;
   const size_t need = ws_bytes(a.b, hd, nt, n_sm);
   if (need && (!r.workspace_dev || r.workspace_bytes < (long long)need))
     return bad("the workspace is smaller than bfp200_kv4_attention_workspace says");
-  float* ws = static_cast<float*>(r.workspace_dev);
+  void* const ws = r.workspace_dev;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = r.dtype == BFP200_F32 ? by_hd<float>(hd, a, nt, n_sm, ws, s)
-                      : r.dtype == BFP200_F16 ? by_hd<__half>(hd, a, nt, n_sm, ws, s)
-                                              : by_hd<__nv_bfloat16>(hd, a, nt, n_sm, ws, s);
+  const cudaError_t e = r.dtype == BFP200_F32 ? by_hd<float>(hd, a, nt, n_sm, spin, ws, s)
+                      : r.dtype == BFP200_F16 ? by_hd<__half>(hd, a, nt, n_sm, spin, ws, s)
+                                              : by_hd<__nv_bfloat16>(hd, a, nt, n_sm, spin, ws, s);
   if (e != cudaSuccess) return bfp200_set_error(BFP200_ECUDA, std::string(who) + ": " + cudaGetErrorString(e));
   return BFP200_OK;
+}
+
+}  // namespace
+}  // namespace kv4
+}  // namespace bfp
+
+using namespace bfp::kv4;
+
+extern "C" int bfp200_kv4_attention_workspace(const bfp200_kv4_attention_args* in, size_t* bytes) {
+  const char* who = "kv4_attention_workspace";
+  const auto bad = [&](const char* what) { return bfp200_set_error(BFP200_EINVAL, std::string(who) + ": " + what); };
+  if (!in || !bytes) return bad("no arguments");
+  Batch b;
+  if (int rc = fill_batch(in->batch, &b, who)) return rc;
+  if (in->H_Q < 1 || in->H_Q % b.H) return bad("H_Q must be a positive multiple of H_KV");
+  int n_sm = 0;
+  if (int rc = device_ready(who, &n_sm)) return rc;
+  const int hd = (int)in->batch.HD;
+  *bytes = b.T == 0 ? 0 : ws_bytes(b, hd, pick_nt(b, (int)in->H_Q / b.H, hd, in->dtype == BFP200_F32), n_sm);
+  return BFP200_OK;
+}
+
+extern "C" int bfp200_kv4_attention_dev(const bfp200_kv4_attention_args* in, void* stream) try {
+  return attention("kv4_attention_dev", in, false, stream);
+} catch (const std::exception& ex) {
+  return bfp200_set_error(BFP200_ENOMEM, ex.what());
+}
+
+extern "C" int bfp200_kv4_wait_probe(const bfp200_kv4_attention_args* in, void* stream) try {
+  return attention("kv4_wait_probe", in, true, stream);
+} catch (const std::exception& ex) {
+  return bfp200_set_error(BFP200_ENOMEM, ex.what());
+}
+
+extern "C" int bfp200_kv4_attention_status(const void* workspace_dev, void* stream) try {
+  const char* who = "kv4_attention_status";
+  if (reinterpret_cast<uintptr_t>(workspace_dev) % 16) return bfp200_set_error(BFP200_EINVAL, std::string(who) + ": misaligned pointer");
+  int n_sm = 0, code = BFP200_OK;
+  if (int rc = device_ready(who, &n_sm)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = workspace_dev ? cudaMemcpyAsync(&code, workspace_dev, sizeof(code), cudaMemcpyDeviceToHost, s) : cudaSuccess;
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess) return bfp200_set_error(BFP200_ECUDA, std::string(who) + ": " + cudaGetErrorString(e));
+  return code == BFP200_OK ? BFP200_OK : bfp200_set_error(BFP200_ETIMEOUT, std::string(who) + ": a bounded device wait timed out");
 } catch (const std::exception& ex) {
   return bfp200_set_error(BFP200_ENOMEM, ex.what());
 }

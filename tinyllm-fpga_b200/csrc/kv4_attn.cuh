@@ -22,7 +22,14 @@ constexpr float V_UP = 16.f;       // V is held times 2^-4
 struct Cut {
   int parts;                       // 0: none
   int q0, rows, r0, head0;         // first token, rows, first row, first query head
-  int pad[3];
+  int late;                        // a wait of the CTA ran out
+  int pad[2];
+};
+
+// The workspace: the call's status, a Cut a CTA, partial sums.
+struct Status {
+  int code;                        // BFP200_OK or BFP200_ETIMEOUT, written by the joining launch
+  int pad[7];
 };
 
 struct AttnArgs {
@@ -32,6 +39,7 @@ struct AttnArgs {
   float* lse;                      // [T][HQ] or null
   float* part;                     // partial sums: [CTA][2][NR][HD + 2]
   Cut* cuts;                       // [CTA]: the item that the CTA begins and does not end
+  Status* status;
   long long q_ts, q_hs, o_ts, o_hs;
   int HQ, group, causal;
   long long window;                // 0: none
@@ -202,13 +210,20 @@ __device__ __forceinline__ void cp16(unsigned d, const void* g) {
 namespace {
 
 // Joins the partial sums of the item that CTA blockIdx.x began and others
-// ended, part after part in their order.
+// ended, part after part in their order.  The last CTA, which can have begun
+// none, gathers the call's status.
 template <typename T, int HD, int NR>
 __global__ void __launch_bounds__(256) join_kernel(const AttnArgs a) {
   constexpr int Q = HD / 4, NG = 256 / Q;          // NG groups of threads share the parts
   __shared__ float4 s_o[NG][Q];
   __shared__ float s_m[NG], s_l[NG];
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (blockIdx.x + 1 == gridDim.x && blockIdx.y == 0) {
+    int late = 0;
+    for (int c = threadIdx.x; c < a.grid; c += 256) late |= __ldcg(&a.cuts[c].late);
+    late = __syncthreads_or(late);
+    if (threadIdx.x == 0) a.status->code = late ? BFP200_ETIMEOUT : BFP200_OK;
+  }
   const int4 c0 = __ldcg(reinterpret_cast<const int4*>(a.cuts + blockIdx.x));
   const int n = c0.x, rows = c0.z;
   if (n == 0) return;
@@ -278,7 +293,9 @@ cudaError_t launch_join(const AttnArgs& a, int rows_at_once, cudaStream_t s) {
 }  // namespace
 
 // The prompt kernel (kv4_prompt.cu): 256 rows a tile on the tensor-memory MMAs.
-template <typename T, int HD> cudaError_t launch_prompt(AttnArgs a, int n_sm, float* ws, cudaStream_t s);
+// Its waits give up after `spin` tries.
+constexpr int SPIN = 1 << 20;
+template <typename T, int HD> cudaError_t launch_prompt(AttnArgs a, int n_sm, int spin, void* ws, cudaStream_t s);
 size_t prompt_ws_bytes(int hd, int n_sm);
 
 }  // namespace kv4

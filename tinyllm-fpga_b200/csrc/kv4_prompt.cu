@@ -22,6 +22,11 @@
 // addresses: 925 us against 863); one warp for both tiles' MMAs (818 against 713
 // with one a tile); one lane polling the barriers for its warp (1075: slower).
 //
+// Waits are bounded.  When one runs out its CTA stops its work, waits for the
+// MMAs in flight, marks the rows that it owes with NaN (a cut item's by the sum
+// that its joining divides by) and leaves a note from which the joining launch
+// makes the call's status.
+//
 // Order.  A tile's MMAs come from one thread, and the scores that overwrite a P
 // are issued behind the product that reads it: the tensor pipe takes them in turn.
 //
@@ -31,7 +36,6 @@
 // rearrangement.  Operands lie as 8-row x 16-byte core matrices without
 // swizzle: [contraction / 8][row][8], which the decoding lanes write 16 bytes
 // at a time to 8 different bank groups.
-#include "kernels.cuh"
 #include "kv4_attn.cuh"
 
 namespace bfp {
@@ -45,7 +49,6 @@ constexpr int MIN_SHARE = 8;                 // blocks that are not worth a seco
 // heads of 128: 730 us at 3, 646 at 6, 666 at 9).
 constexpr int ITEM = 6;
 constexpr int THREADS = 512;                  // softmax 2 x 4 warps, decoding 4, MMA 2, rows of no sequence 2
-constexpr int SPIN = 1 << 20;
 
 __device__ __forceinline__ void mb_init(unsigned long long* bar, unsigned count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(su32(bar)), "r"(count) : "memory");
@@ -340,7 +343,7 @@ __device__ __forceinline__ float row_weights(uint32_t (&ph)[32 * PS], const uint
 template <int HD> constexpr int SMEM = 2 * 128 * HD * 2 + 4 * PB * HD * 2;   // queries of two tiles, two stages of keys and of values
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, int* err, int q_vec, int o_vec) {
+__global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, int spin, int q_vec, int o_vec) {
   constexpr int KU = HD / 32, REC9 = HD * 9 / 8, PS = Kind<T>::PS;
   constexpr bool HALF_K = Kind<T>::HALF_K;
   constexpr int TILE_Q = 128 * HD * 2, TILE_KV = PB * HD * 2;
@@ -359,7 +362,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
     }
     mb_init(&drained, 2);
     s_abort = 0;
-    a.cuts[blockIdx.x].parts = 0;
+    a.cuts[blockIdx.x] = Cut{};
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 12) {
@@ -371,12 +374,11 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
   tc_after();
   const uint32_t tmem = s_tmem;
   const auto wait = [&](unsigned long long* bar, unsigned parity) -> bool {
-    for (int it = 0; it < SPIN; ++it) {
+    for (int it = 0; it < spin; ++it) {
       if (mb_try(bar, parity)) return true;
       if (s_abort) return false;
     }
     s_abort = 1;
-    atomicExch(err, 6);
     return false;
   };
 
@@ -386,14 +388,15 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
   const int page = a.b.page, rec_bytes = page * REC9;
   const long long page_bytes = (long long)rec_bytes * a.b.H;
   bool ok = true;
-  // A CTA's share, item by item; every role walks through it by itself.
+  // A CTA's share, item by item; every role walks through it by itself, also
+  // when a wait has run out (!ok): then there are still rows to be marked.
   const auto share = [&](auto role) {
     if ((long long)blockIdx.x >= plan.geff || plan.total == 0) return;
     Seg g;
     g.nk = g.nt1 = g.seg0 = g.seg1 = 0;
     g.x = bound_of(a, plan, blockIdx.x);
     const long long x1 = bound_of(a, plan, (long long)blockIdx.x + 1);
-    while (g.x < x1 && ok) {
+    while (g.x < x1) {
       g.it = item_of(a, plan, g.x);
       g.xe = min(x1, g.it.end);
       if (g.xe <= g.x) break;                                // lengths changed during the call
@@ -423,6 +426,17 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
   if (warp < 8) {
     // ================= softmax: one thread a row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    // a row that a wait left undone: NaN, in its output or in the sum that its joining divides by
+    const auto not_done = [&](bool live, bool full, T* dst, float* part, int pr, int token, int head) {
+      if (live && full) {
+        #pragma unroll 1
+        for (int d = 0; d < HD; ++d) dst[d] = from_f<T>(NAN);
+        if (a.lse) a.lse[(long long)token * a.HQ + head] = NAN;
+      } else if (live) {
+        part[PR * HD + pr] = -INFINITY;
+        part[PR * HD + PR + pr] = NAN;
+      }
+    };
     share([&](const Seg& g) {
       const int tile = warp >> 2, n = g.n, blk0 = g.blk0, r0 = g.r0, rows = g.rows;
       if (tile == 0 || rows > 128) {
@@ -434,6 +448,14 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
         const int blocks0 = tile ? g.nt1 : g.nk, seg = tile ? g.seg1 : g.seg0;
         // queries: [dim / 8][row][dims 0 4 1 5 2 6 3 7]
         const T* q = static_cast<const T*>(a.q) + (long long)(q0 + j) * a.q_ts + (long long)head * a.q_hs;
+        const bool full = g.x == g.it.start && g.xe == g.it.end;
+        T* const dst = static_cast<T*>(a.out) + (long long)(q0 + j) * a.o_ts + (long long)head * a.o_hs;
+        float* const part = a.part + ((long long)blockIdx.x * 2 + (g.x > g.it.start ? 0 : 1)) * PR * (HD + 2);
+        const int pr = tile * 128 + row;
+        if (!ok) {
+          not_done(live, full, dst, part, pr, q0 + j, head);
+          return;
+        }
         uint4 qv[HD / 8];
         #pragma unroll
         for (int c = 0; c < HD / 8; ++c) {                  // (all of the row's loads at once)
@@ -515,11 +537,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
         }
         if (ok && (ok = warp_wait(&ofull[tile][1], seg & 1))) {
           tc_after();
-          const bool full = g.x == g.it.start && g.xe == g.it.end;
           const float inv = l == 0.f ? 0.f : V_UP / l;
-          T* dst = static_cast<T*>(a.out) + (long long)(q0 + j) * a.o_ts + (long long)head * a.o_hs;
-          float* part = a.part + ((long long)blockIdx.x * 2 + (g.x > g.it.start ? 0 : 1)) * PR * (HD + 2);
-          const int pr = tile * 128 + row;
           #pragma unroll 1
           for (int c = 0; c < HD / 32; ++c) {
             uint32_t o[32];
@@ -544,6 +562,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
             part[PR * HD + pr] = m * a.scale_log2;
             part[PR * HD + PR + pr] = l;
           }
+        } else {
+          not_done(live, full, dst, part, pr, q0 + j, head);
         }
       }
     });
@@ -606,7 +626,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
       fetch_v(blk0 * PB, page_at(b0 + 8 * vo));
       int pk = -1, pv = -1;
       if (n > 1) { pk = page_at(b0 + PB + 4 * kq); pv = page_at(b0 + PB + 8 * vo); }
-      for (int i = 0; i < n; ++i) {
+      for (int i = 0; i < n && ok; ++i) {
         const int kc = nk + i, st = kc & 1;
         // keys
         if (kc >= 2 && !(ok = warp_wait(&kfree[st], ((kc >> 1) + 1) & 1))) break;
@@ -665,7 +685,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
         const long long c = blockIdx.x;
         long long e = min(plan.geff, div_small(g.it.end * plan.geff + plan.total - 1, plan.total));
         while (e - 1 > c + 1 && bound_of(a, plan, e - 1) >= g.it.end) --e;
-        if (lane == 0) a.cuts[c] = Cut{(int)(e - c), g.it.q.q0, g.rows, g.r0, g.it.head * a.group, {0, 0, 0}};
+        if (lane == 0) a.cuts[c] = Cut{(int)(e - c), g.it.q.q0, g.rows, g.r0, g.it.head * a.group, 0, {0, 0}};
       }
     });
   } else {
@@ -674,6 +694,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
     // tile's lie under the other's MMAs.)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp < 14) share([&](const Seg& g) {
+      if (!ok) return;
       const int n = g.n, nk = g.nk, t = warp - 12;
       const bool both = g.rows > 128;
       if (t && !both) {
@@ -742,6 +763,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
   }
   tc_before();
   __syncthreads();
+  if (tid == 0) a.cuts[blockIdx.x].late = s_abort;
   if (warp == 12) {
     tc_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(512) : "memory");
@@ -750,32 +772,31 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
 
 }  // namespace
 
-size_t prompt_ws_bytes(int hd, int n_sm) { return (size_t)n_sm * (sizeof(Cut) + 2 * PR * (hd + 2) * 4); }
+size_t prompt_ws_bytes(int hd, int n_sm) { return sizeof(Status) + (size_t)n_sm * (sizeof(Cut) + 2 * PR * (hd + 2) * 4); }
 
 template <typename T, int HD>
-cudaError_t launch_prompt(AttnArgs a, int n_sm, float* ws, cudaStream_t s) {
+cudaError_t launch_prompt(AttnArgs a, int n_sm, int spin, void* ws, cudaStream_t s) {
   auto* kern = prompt_kernel<T, HD>;
   static std::atomic<unsigned char> allowed[128];
   cudaError_t e = allow_smem(kern, SMEM<HD>, allowed);
   if (e != cudaSuccess) return e;
-  int* err = error_flag_device_ptr();
-  if (!err) return cudaErrorInvalidSymbol;
   a.grid = n_sm;
-  a.cuts = reinterpret_cast<Cut*>(ws);
+  a.status = static_cast<Status*>(ws);
+  a.cuts = reinterpret_cast<Cut*>(a.status + 1);
   a.part = reinterpret_cast<float*>(a.cuts + a.grid);
   const auto vec = [](const void* p, long long ts, long long hs) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ts % 8 == 0 && hs % 8 == 0 ? 1 : 0;
   };
-  kern<<<a.grid, THREADS, SMEM<HD>, s>>>(a, err, vec(a.q, a.q_ts, a.q_hs), vec(a.out, a.o_ts, a.o_hs));
+  kern<<<a.grid, THREADS, SMEM<HD>, s>>>(a, spin, vec(a.q, a.q_ts, a.q_hs), vec(a.out, a.o_ts, a.o_hs));
   e = cudaGetLastError();
   return e == cudaSuccess ? launch_join<T, HD, PR>(a, 16, s) : e;
 }
 
 #define BFP200_PROMPT(T) \
-  template cudaError_t launch_prompt<T, 32>(AttnArgs, int, float*, cudaStream_t); \
-  template cudaError_t launch_prompt<T, 64>(AttnArgs, int, float*, cudaStream_t); \
-  template cudaError_t launch_prompt<T, 96>(AttnArgs, int, float*, cudaStream_t); \
-  template cudaError_t launch_prompt<T, 128>(AttnArgs, int, float*, cudaStream_t);
+  template cudaError_t launch_prompt<T, 32>(AttnArgs, int, int, void*, cudaStream_t); \
+  template cudaError_t launch_prompt<T, 64>(AttnArgs, int, int, void*, cudaStream_t); \
+  template cudaError_t launch_prompt<T, 96>(AttnArgs, int, int, void*, cudaStream_t); \
+  template cudaError_t launch_prompt<T, 128>(AttnArgs, int, int, void*, cudaStream_t);
 BFP200_PROMPT(__nv_bfloat16)
 BFP200_PROMPT(__half)
 
