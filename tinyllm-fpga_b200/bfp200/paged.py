@@ -65,8 +65,12 @@ class PagedDecoder:
         return ops.rmsnorm_fp(h, self.norm_w, cfg.eps) @ self.emb.T
 
     def generate(self, prompts, n_gen):
-        """prompt + n_gen greedy ids per sequence."""
+        """prompt + n_gen greedy ids per sequence (of no sequences, none)."""
         lens = [len(p) for p in prompts]
+        if not lens:
+            return []
+        if min(lens) < 1:
+            raise ValueError("a prompt needs at least one id")
         need = [-(-(n + n_gen) // self.page) for n in lens]
         if sum(need) > len(self.free):
             raise ValueError(f"{sum(need)} pages are needed, {len(self.free)} are free")
