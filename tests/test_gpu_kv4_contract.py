@@ -246,3 +246,20 @@ def test_the_status_of_calls_without_waits():
         assert _raw_attention("bfp200_kv4_attention_dev", case, q, out, lse, ws) == _lib.OK
         assert L.bfp200_kv4_attention_status(ws.data_ptr(), stream) == _lib.OK
         kv4.attention(q, case.pool, case.q_start, case.len_t, case.bt, check_done=True)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 63 - 1])
+@pytest.mark.parametrize("HD,group,new", FORMS)
+def test_attention_windows_wider_than_any_position(HD, group, new, window, dtype):
+    """As without a window, also for tokens before their sequence and far past its table."""
+    import torch
+    from bfp200 import kv4
+    rng = np.random.default_rng(HD)
+    case = Case(rng, [112, 112, 112], [new] * 3, 2, HD, 16, extra_cols=0)      # whole pages: the last length claims them all
+    lens = _i32([new // 2, 112, 10 ** 9])
+    q = _rand(rng, (3 * new, 2 * group, HD), dtype)
+    for causal in (True, False):
+        want = kv4.attention(q, case.pool, case.q_start, lens, case.bt, causal=causal, return_lse=True)
+        got = kv4.attention(q, case.pool, case.q_start, lens, case.bt, causal=causal, window=window, return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -756,7 +756,7 @@ int attention(const char* who, const bfp200_kv4_attention_args* in, bool probe, 
   a.HQ = (int)r.H_Q;
   a.group = a.HQ / a.b.H;
   a.causal = r.causal != 0;
-  a.window = r.window;
+  a.window = r.window < (1LL << 31) ? r.window : 1LL << 31;   // (hides nothing; what the kernels add to it stays in range)
   const double sl = std::fabs(r.scale) * 1.4426950408889634 * (r.dtype == BFP200_F16 ? 16.0 : 1.0);   // K is held times 2^-4 there
   if (sl > 1e30) return bad("scale is too large");
   a.scale_log2 = (float)std::fmax(sl, 1e-30);
