@@ -22,3 +22,37 @@ def test_paged_generate_refuses_empty_prompts(prompts):
 
 def test_paged_generate_of_no_prompts():
     assert _paged().generate([], 3) == []
+
+
+def _batch(**kw):
+    d = dict(pool=4096, bt=4096, qs=4096, lens=4096, n_pages=4, page=16, H=2, HD=64, n=1, cols=2, ld=2, T=2)
+    d.update(kw)
+    return tuple(d.values())
+
+
+def _calls(batch):
+    """read, append, attention and its workspace with these words of the batch."""
+    from bfp200 import _lib, kv4
+    L = _lib.lib()
+    att = kv4._ATTENTION.pack(*batch, *[4096] * 4, 1 << 30, *[64] * 4, 4, 0, 1, 0, 0.125)
+    return (L.bfp200_kv4_read_dev(kv4._READ.pack(*batch, 4096, 4096, 0), None),
+            L.bfp200_kv4_append_dev(kv4._APPEND.pack(*batch, *[4096] * 4, *[64] * 8, 0, 0, 2, 0, 0, 0, 0), None),
+            L.bfp200_kv4_attention_dev(att, None), L.bfp200_kv4_attention_workspace(att, _lib.C.c_size_t()))
+
+
+@pytest.mark.parametrize("which", ["bt", "qs", "lens"])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_misaligned_batch_arrays_are_refused(which, off):
+    """The kernels read them as 32-bit words, which at other addresses would be a fault of the GPU."""
+    from bfp200 import _lib
+    assert _calls(_batch(**{which: 4096 + off})) == (_lib.EINVAL,) * 4
+    assert "aligned" in _lib.last_error()
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_misaligned_positions_are_refused(off):
+    from bfp200 import _lib, kv4
+    L = _lib.lib()
+    for rc in (L.bfp200_rope_dev(kv4._ROPE.pack(4096, 4096, 4096, 4096 + off, 64, 64, 64, 64, 2, 2, 64, 8, 64, 0, 0, 0), None),
+               L.bfp200_kv4_append_dev(kv4._APPEND.pack(*_batch(), *[4096] * 4, *[64] * 8, 4096, 4096 + off, 2, 64, 64, 0, 0), None)):
+        assert rc == _lib.EINVAL and "aligned" in _lib.last_error()

@@ -54,6 +54,9 @@ int fill_batch(const bfp200_kv4_batch& in, Batch* out, const char* who) {
   if (in.n_tokens > 0 && in.n_seq > 0 && in.max_pages > 0 && !in.block_table_dev) return bad("the block table is needed");
   if (in.n_pages > 0 && !in.pool_dev) return bad("the pool is needed");
   if (reinterpret_cast<uintptr_t>(in.pool_dev) & 15u) return bad("the pool must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(in.q_start_dev) | reinterpret_cast<uintptr_t>(in.lens_dev) |
+       reinterpret_cast<uintptr_t>(in.block_table_dev)) & 3u)
+    return bad("q_start, lens and the block table must be 4-byte aligned");
   out->pool = static_cast<uint8_t*>(in.pool_dev);
   out->bt = in.block_table_dev;
   out->q_start = in.q_start_dev;
@@ -595,6 +598,7 @@ extern "C" int bfp200_rope_dev(const bfp200_rope_args* in, void* stream) try {
   if (!r.T || !r.H) return BFP200_OK;
   if (!r.x_dev || !r.out_dev || !r.positions_dev || (r.rot && !r.table_dev)) return bad("null pointer");
   if (reinterpret_cast<uintptr_t>(r.table_dev) & 7u) return bad("the table must be 8-byte aligned");
+  if (reinterpret_cast<uintptr_t>(r.positions_dev) & 3u) return bad("positions must be 4-byte aligned");
   const int es = elem_size(r.dtype);
   if ((reinterpret_cast<uintptr_t>(r.x_dev) | reinterpret_cast<uintptr_t>(r.out_dev)) % es) return bad("misaligned x or out");
   int n_sm = 0;
@@ -630,6 +634,7 @@ extern "C" int bfp200_kv4_append_dev(const bfp200_kv4_append_args* in, void* str
     if (!r.positions_dev && r.n_pos < r.batch.max_pages * r.batch.page)
       return bad("the rotation table is shorter than max_pages * page positions");
     if (reinterpret_cast<uintptr_t>(r.table_dev) & 7u) return bad("the table must be 8-byte aligned");
+    if (reinterpret_cast<uintptr_t>(r.positions_dev) & 3u) return bad("positions must be 4-byte aligned");
   }
   if (a.b.T == 0 || (a.b.n_seq == 0 && r.H_Q == 0)) return BFP200_OK;
   if (!r.k_dev || !r.v_dev || (r.H_Q > 0 && (!r.q_dev || !r.q_out_dev))) return bad("null pointer");
