@@ -56,3 +56,11 @@ def test_misaligned_positions_are_refused(off):
     for rc in (L.bfp200_rope_dev(kv4._ROPE.pack(4096, 4096, 4096, 4096 + off, 64, 64, 64, 64, 2, 2, 64, 8, 64, 0, 0, 0), None),
                L.bfp200_kv4_append_dev(kv4._APPEND.pack(*_batch(), *[4096] * 4, *[64] * 8, 4096, 4096 + off, 2, 64, 64, 0, 0), None)):
         assert rc == _lib.EINVAL and "aligned" in _lib.last_error()
+
+
+@pytest.mark.parametrize("cols,page", [(1 << 60, 16), ((1 << 60) + 5, 16), (1 << 55, 256), ((1 << 63) - 1, 256), ((1 << 26) + 1, 16)])
+def test_tables_of_too_many_positions_are_refused(cols, page):
+    """Also where max_pages * page passes 64 bits."""
+    from bfp200 import _lib
+    assert _calls(_batch(cols=cols, page=page, pool=4096)) == (_lib.EINVAL,) * 4
+    assert "2^30 positions" in _lib.last_error()

@@ -49,7 +49,7 @@ int fill_batch(const bfp200_kv4_batch& in, Batch* out, const char* who) {
   if (in.H_KV < 1 || in.H_KV > 1024) return bad("H_KV must be 1..1024");
   if (in.n_tokens > (1LL << 30) || in.n_seq > (1LL << 24) || in.n_pages > (1LL << 30))
     return bad("too many tokens, sequences or pages");
-  if (in.max_pages * in.page > (1LL << 30)) return bad("a sequence may hold at most 2^30 positions");
+  if (in.max_pages > (1LL << 30) / in.page) return bad("a sequence may hold at most 2^30 positions");
   if (in.n_tokens > 0 && in.n_seq > 0 && (!in.q_start_dev || !in.lens_dev)) return bad("q_start and lens are needed");
   if (in.n_tokens > 0 && in.n_seq > 0 && in.max_pages > 0 && !in.block_table_dev) return bad("the block table is needed");
   if (in.n_pages > 0 && !in.pool_dev) return bad("the pool is needed");
