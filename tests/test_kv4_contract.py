@@ -64,3 +64,15 @@ def test_tables_of_too_many_positions_are_refused(cols, page):
     from bfp200 import _lib
     assert _calls(_batch(cols=cols, page=page, pool=4096)) == (_lib.EINVAL,) * 4
     assert "2^30 positions" in _lib.last_error()
+
+
+def test_no_exception_leaves_a_c_entry_point():
+    """Each one is a function-try-block: an error message that finds no memory becomes a code."""
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tinyllm-fpga_b200", "csrc")
+    heads = []
+    for name in ("kv4.cu", "kv4_attn.cu", "kv4_prompt.cu"):
+        with open(os.path.join(csrc, name)) as f:
+            heads += re.findall(r'^extern "C" int (\w+)\([^)]*\) *(\w*)', f.read(), re.M)
+    assert len(heads) >= 7 and [h for h, word in heads if word != "try"] == []

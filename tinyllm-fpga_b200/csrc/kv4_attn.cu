@@ -786,7 +786,7 @@ int attention(const char* who, const bfp200_kv4_attention_args* in, bool probe, 
 
 using namespace bfp::kv4;
 
-extern "C" int bfp200_kv4_attention_workspace(const bfp200_kv4_attention_args* in, size_t* bytes) {
+extern "C" int bfp200_kv4_attention_workspace(const bfp200_kv4_attention_args* in, size_t* bytes) try {
   const char* who = "kv4_attention_workspace";
   const auto bad = [&](const char* what) { return bfp200_set_error(BFP200_EINVAL, std::string(who) + ": " + what); };
   if (!in || !bytes) return bad("no arguments");
@@ -798,6 +798,8 @@ extern "C" int bfp200_kv4_attention_workspace(const bfp200_kv4_attention_args* i
   const int hd = (int)in->batch.HD;
   *bytes = b.T == 0 ? 0 : ws_bytes(b, hd, pick_nt(b, (int)in->H_Q / b.H, hd, in->dtype == BFP200_F32), n_sm);
   return BFP200_OK;
+} catch (const std::exception& ex) {
+  return bfp200_set_error(BFP200_ENOMEM, ex.what());
 }
 
 extern "C" int bfp200_kv4_attention_dev(const bfp200_kv4_attention_args* in, void* stream) try {
