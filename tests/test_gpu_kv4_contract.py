@@ -263,3 +263,31 @@ def test_attention_windows_wider_than_any_position(HD, group, new, window, dtype
         want = kv4.attention(q, case.pool, case.q_start, lens, case.bt, causal=causal, return_lse=True)
         got = kv4.attention(q, case.pool, case.q_start, lens, case.bt, causal=causal, window=window, return_lse=True)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("inter,inverse", [(False, False), (True, False), (False, True)])
+def test_rope_hands_its_gradient_on(inter, inverse, dtype):
+    """A tensor that requires a gradient gets it, the inverse turn of the
+    output's, from a gradient with any strides; the second derivative is the
+    turn again."""
+    import torch
+    from bfp200 import kv4
+    rng = np.random.default_rng(2)
+    table, pos = kv4.rope_table(100, 48), _i32([3, 99, 41])
+    turn = lambda x, inv: kv4.rope(x, pos, table, interleaved=inter, inverse=inv)
+    x = _rand(rng, (3, 2, 96), dtype).requires_grad_()
+    g = _rand(rng, (3, 2, 96), dtype)
+    y = turn(x, inverse)
+    assert y.requires_grad and torch.equal(y.detach(), turn(x.detach(), inverse))
+    for grad in (g, g.transpose(0, 1).contiguous().transpose(0, 1), g.transpose(1, 2).contiguous().transpose(1, 2), g[:1, :1, :1].expand(3, 2, 96)):
+        got, = torch.autograd.grad(y, x, grad, retain_graph=True)
+        assert torch.equal(got, turn(grad.contiguous(), not inverse))
+    y.sum().backward()
+    assert torch.equal(x.grad, turn(torch.ones_like(g), not inverse))
+    h = g.clone().requires_grad_()
+    first, = torch.autograd.grad(turn(x, inverse), x, h, create_graph=True)
+    second, = torch.autograd.grad(first, h, g)
+    assert torch.equal(second, turn(g, inverse))
+    with torch.no_grad():
+        assert not turn(x, inverse).requires_grad

@@ -14,6 +14,9 @@ needs no copy).  The C entry points are ``bfp200_rope_dev`` and
 ``bfp200_kv4_*_dev`` of include/bfp200.h, which also defines the bytes of the
 cache: BFP tiles of 16 head dims, 4-bit mantissas, one exponent byte.
 
+Rotation passes gradients on; append, read and attention have no backward pass,
+and what they return carries no gradient.
+
 A batch is three int32 tensors: ``lens[s]`` positions of sequence s, held in
 pages ``block_table[s, 0..]``; ``q_start[s] .. q_start[s + 1]`` its rows among
 this call's tokens, which are its last positions.  They are read on the
@@ -200,7 +203,10 @@ def rope(x, positions, table, interleaved=False, inverse=False, out=None):
     """x [tokens, heads, HD] with the first rot = 2 * table.shape[1] dims of
     every head turned by its token's angles: pairs (j, j + rot / 2), or (2 j,
     2 j + 1) if interleaved; the other dims are copied.  inverse turns back,
-    which is the gradient of the forward turn.  out may be x."""
+    which is the gradient of the forward turn: an x that requires a gradient
+    gets it so.  out may be x; a result in out carries no gradient."""
+    if out is None and x.requires_grad and torch.is_grad_enabled():
+        return _Rope.apply(x, positions, table, interleaved, inverse)
     dev, code, t, h, d, xt, xh = _acts(x, "x")
     if out is None:
         out = x.new_empty((t, h, d))
@@ -212,6 +218,23 @@ def rope(x, positions, table, interleaved=False, inverse=False, out=None):
     _run(_fn("bfp200_rope_dev"), _ROPE.pack(x.data_ptr(), out.data_ptr(), tp, pp, xt, xh, ot, oh, t, h, d, n_pos, rot, code,
                                             interleaved, inverse), dev)
     return out
+
+
+class _Rope(torch.autograd.Function):
+    """rope of an x that requires a gradient."""
+
+    @staticmethod
+    def forward(ctx, x, positions, table, interleaved, inverse):
+        ctx.save_for_backward(positions, table)
+        ctx.form = interleaved, inverse
+        return rope(x, positions, table, interleaved, inverse)
+
+    @staticmethod
+    def backward(ctx, g):
+        positions, table = ctx.saved_tensors
+        interleaved, inverse = ctx.form
+        g = g if g.stride(-1) == 1 else g.contiguous()
+        return rope(g, positions, table, interleaved, not inverse), None, None, None, None
 
 
 def append(pool, k, v, q_start, lens, block_table, q=None, table=None, interleaved=False, positions=None, q_out=None):
