@@ -291,3 +291,27 @@ def test_rope_hands_its_gradient_on(inter, inverse, dtype):
     assert torch.equal(second, turn(g, inverse))
     with torch.no_grad():
         assert not turn(x, inverse).requires_grad
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("n,HD,group,window", [(300, 128, 4, 0), (700, 128, 4, 20), (300, 32, 12, 0)])
+def test_attention_prompts_of_many_sequences(n, HD, group, window, dtype):
+    """The prompts' kernel over more than 256 sequences, whose schedule is kept
+    in chunks of several: among them sequences without tokens, without
+    positions and with fewer positions than tokens."""
+    from bfp200 import kv4
+    rng = np.random.default_rng(n + window)
+    lens, news = rng.integers(0, 60, n), rng.integers(0, 26 if HD > 64 else 64, n)
+    news[rng.integers(0, n, n // 10)] = 0
+    lens[rng.integers(0, n, n // 10)] = 0
+    case = Case(rng, lens, news, 1, HD, 16)
+    assert case.tokens * group > (32 if HD > 64 else 256) * n     # enough rows a sequence for that kernel
+    q = _rand(rng, (case.tokens, group, HD), dtype)
+    out, lse = kv4.attention(q, case.pool, case.q_start, case.len_t, case.bt, window=window, return_lse=True)
+    t = 0
+    for s in range(n):
+        L, m = int(lens[s]), int(news[s])
+        rows = slice(t, t + m)
+        t += m
+        if m:
+            _check_rows(q[rows], *case.kv[s], _visible(L - m + np.arange(m), L, True, window), out[rows], lse[rows], dtype)
