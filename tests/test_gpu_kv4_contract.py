@@ -315,3 +315,17 @@ def test_attention_prompts_of_many_sequences(n, HD, group, window, dtype):
         t += m
         if m:
             _check_rows(q[rows], *case.kv[s], _visible(L - m + np.arange(m), L, True, window), out[rows], lse[rows], dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_append_of_lowest_and_highest_mantissas(dtype):
+    """Words whose nibbles are all 0 (mantissa -8, a sum below -2^31) or all 15."""
+    import torch
+    from bfp200 import kv4
+    pool = kv4.new_pool(1, 1, 64, 16)
+    k = torch.full((2, 1, 64), -1.99, device="cuda", dtype=_dt(dtype))
+    k[1] = 1.99
+    args = (pool, _i32([0, 2]), _i32([2]), _i32([[0]]))
+    kv4.append(args[0], k, k, *args[1:])
+    rk, rv = kv4.read(*args, 2, dtype=torch.float32)
+    assert (rk[0] == -2.0).all() and (rk[1] == 1.75).all() and torch.equal(rk, rv)

@@ -379,10 +379,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) append_kernel(con
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     e = tile_e(top);
     const float up = pow2f(3 - e);
-    int w = 0;                                              // sum of m_i 16^i; adding 8 to every nibble makes them 0..15
+    unsigned w = 0;                                         // sum of m_i 16^i modulo 2^32; adding 8 to every nibble makes them 0..15
     #pragma unroll
-    for (int i = 7; i >= 0; --i) w = w * 16 + mantissa(f[i], up);
-    return (unsigned)w + 0x88888888u;
+    for (int i = 7; i >= 0; --i) w = w * 16 + (unsigned)mantissa(f[i], up);
+    return w + 0x88888888u;
   };
   const int slot = pos & (a.b.page - 1), page = a.b.page;
   uint8_t* const rec0 = a.b.pool + (store ? (long long)pg * H : 0) * (page * REC9);
