@@ -148,6 +148,13 @@ struct Item {
   Seq q;
 };
 
+// What a CTA needs again behind an item's loop, which leaves no registers for it.
+struct Held {
+  Item it;
+  long long x, xe, x1;             // the CTA's blocks of the item, the end of its share
+  int h, r0, rows;
+};
+
 // The item that holds block x (0 <= x < total).
 template <int NR, int BLK>
 __device__ Item item_at(const AttnArgs& a, const Sched& s, long long x) {
@@ -252,14 +259,18 @@ __global__ void __launch_bounds__(Shape<HD, NT>::W * 32, Shape<HD, NT>::CTAS) at
   float* s_m = s_o + W * NR * HD;                                     // [W][NR], [W][NR]
   float* s_l = s_m + W * NR;
   __shared__ Sched sch;
+  __shared__ Held held;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   make_sched<NR, BLK, W * 32>(a, sch);
   clear_rows<T, HD>(a, blockIdx.x * W + warp, gridDim.x * W);
-  if (tid == 0 && a.cuts) a.cuts[blockIdx.x] = Cut{};
+  if (tid == 0 && a.cuts) {
+    a.cuts[blockIdx.x].parts = 0;
+    if (blockIdx.x == 0) a.status->code = BFP200_OK;                    // (no wait here can run out)
+  }
   if ((long long)blockIdx.x >= sch.geff || sch.total == 0) return;
   long long x = bound<NR, BLK>(a, sch, (long long)blockIdx.x + (lane & 1));   // both bounds at once
-  const long long x1 = __shfl_sync(0xffffffffu, x, 1);
+  long long x1 = __shfl_sync(0xffffffffu, x, 1);
   x = __shfl_sync(0xffffffffu, x, 0);
   const int page = a.b.page, rec_bytes = page * REC9;
   const long long page_bytes = (long long)rec_bytes * a.b.H;
@@ -267,10 +278,11 @@ __global__ void __launch_bounds__(Shape<HD, NT>::W * 32, Shape<HD, NT>::CTAS) at
   Item it;
   if (x < x1) it = item_at<NR, BLK>(a, sch, x);
   while (x < x1) {
-    const long long xe = min(x1, it.end);
+    long long xe = min(x1, it.end);
     if (xe <= x) break;                                               // lengths changed during the call
-    const int rt = it.q.rt, h = it.idx / rt, r0 = (it.idx - h * rt) * NR;
-    const int rows = min(NR, it.q.n_q * a.group - r0);
+    const int rt = it.q.rt;
+    int h = it.idx / rt, r0 = (it.idx - h * rt) * NR;
+    int rows = min(NR, it.q.n_q * a.group - r0);
     const int len = it.q.len, qp0 = it.q.qp0;
     // ---- rows: queries to operand registers
     for (int i = tid; i < HD / 16 * NT * 32; i += W * 32) {
@@ -317,6 +329,7 @@ __global__ void __launch_bounds__(Shape<HD, NT>::W * 32, Shape<HD, NT>::CTAS) at
           #pragma unroll
           for (int k = 0; k < 4; ++k) O[w][n][nt][k] = 0.f;
     }
+    if (tid == 0) held = Held{it, x, xe, x1, h, r0, rows};
     __syncthreads();
 
     // this segment's blocks that some row sees, as positions
@@ -594,6 +607,9 @@ __global__ void __launch_bounds__(Shape<HD, NT>::W * 32, Shape<HD, NT>::CTAS) at
       accumulate(vs);
     }
     __syncthreads();                                                  // the rings become the joining buffers
+    it = held.it;
+    x = held.x; xe = held.xe; x1 = held.x1;
+    h = held.h; r0 = held.r0; rows = held.rows;
 
     // ---- join the warps
     #pragma unroll
@@ -689,7 +705,7 @@ cudaError_t launch_attn(AttnArgs a, int n_sm, void* ws, cudaStream_t s) {
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   if (whole) return cudaSuccess;
-  return launch_join<T, HD, NR>(a, 4, s);
+  return launch_join<T, HD, NR, false>(a, 4, s);
 }
 
 // Row tile of a call, by the sequences' average of tokens times the group; 8

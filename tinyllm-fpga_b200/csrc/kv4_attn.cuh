@@ -28,8 +28,8 @@ struct Cut {
 
 // The workspace: the call's status, a Cut a CTA, partial sums.
 struct Status {
-  int code;                        // BFP200_OK or BFP200_ETIMEOUT, written by the joining launch
-  int pad[7];
+  int code;                        // BFP200_OK or BFP200_ETIMEOUT
+  int pad[31];                     // (a line: what follows keeps its alignment)
 };
 
 struct AttnArgs {
@@ -210,15 +210,17 @@ __device__ __forceinline__ void cp16(unsigned d, const void* g) {
 namespace {
 
 // Joins the partial sums of the item that CTA blockIdx.x began and others
-// ended, part after part in their order.  The last CTA, which can have begun
-// none, gathers the call's status.
-template <typename T, int HD, int NR>
+// ended, part after part in their order.  Behind the prompts' kernel it also
+// clears the rows of no sequence, beside that kernel's end, and its last CTA,
+// which can have begun no item, gathers the call's status.
+template <typename T, int HD, int NR, bool PROMPT>
 __global__ void __launch_bounds__(256) join_kernel(const AttnArgs a) {
   constexpr int Q = HD / 4, NG = 256 / Q;          // NG groups of threads share the parts
   __shared__ float4 s_o[NG][Q];
   __shared__ float s_m[NG], s_l[NG];
+  if (PROMPT) clear_rows<T, HD>(a, (blockIdx.y * gridDim.x + blockIdx.x) * 8 + threadIdx.x / 32, gridDim.x * gridDim.y * 8);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (blockIdx.x + 1 == gridDim.x && blockIdx.y == 0) {
+  if (PROMPT && blockIdx.x + 1 == gridDim.x && blockIdx.y == 0) {
     int late = 0;
     for (int c = threadIdx.x; c < a.grid; c += 256) late |= __ldcg(&a.cuts[c].late);
     late = __syncthreads_or(late);
@@ -276,7 +278,7 @@ __global__ void __launch_bounds__(256) join_kernel(const AttnArgs a) {
   }
 }
 
-template <typename T, int HD, int NR>
+template <typename T, int HD, int NR, bool PROMPT>
 cudaError_t launch_join(const AttnArgs& a, int rows_at_once, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.grid, rows_at_once);
@@ -287,7 +289,7 @@ cudaError_t launch_join(const AttnArgs& a, int rows_at_once, cudaStream_t s) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel<T, HD, NR>, a);
+  return cudaLaunchKernelEx(&cfg, join_kernel<T, HD, NR, PROMPT>, a);
 }
 
 }  // namespace

@@ -48,7 +48,7 @@ constexpr int MIN_SHARE = 8;                 // blocks that are not worth a seco
 // An item's queries, first block and outputs, in blocks (8192 tokens, 32 / 8
 // heads of 128: 730 us at 3, 646 at 6, 666 at 9).
 constexpr int ITEM = 6;
-constexpr int THREADS = 512;                  // softmax 2 x 4 warps, decoding 4, MMA 2, rows of no sequence 2
+constexpr int THREADS = 512;                  // softmax 2 x 4 warps, decoding 4, MMA 2 (and 2 that wait at the end)
 
 __device__ __forceinline__ void mb_init(unsigned long long* bar, unsigned count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(su32(bar)), "r"(count) : "memory");
@@ -426,15 +426,18 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
   if (warp < 8) {
     // ================= softmax: one thread a row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    const auto part_of = [&](const Seg& g) { return a.part + ((long long)blockIdx.x * 2 + (g.x > g.it.start ? 0 : 1)) * PR * (HD + 2); };
     // a row that a wait left undone: NaN, in its output or in the sum that its joining divides by
-    const auto not_done = [&](bool live, bool full, T* dst, float* part, int pr, int token, int head) {
-      if (live && full) {
+    const auto not_done = [&](const Seg& g, int row, int token, int head) {
+      if (g.x == g.it.start && g.xe == g.it.end) {
+        T* dst = static_cast<T*>(a.out) + (long long)token * a.o_ts + (long long)head * a.o_hs;
         #pragma unroll 1
         for (int d = 0; d < HD; ++d) dst[d] = from_f<T>(NAN);
         if (a.lse) a.lse[(long long)token * a.HQ + head] = NAN;
-      } else if (live) {
-        part[PR * HD + pr] = -INFINITY;
-        part[PR * HD + PR + pr] = NAN;
+      } else {
+        float* part = part_of(g);
+        part[PR * HD + row] = -INFINITY;
+        part[PR * HD + PR + row] = NAN;
       }
     };
     share([&](const Seg& g) {
@@ -448,12 +451,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
         const int blocks0 = tile ? g.nt1 : g.nk, seg = tile ? g.seg1 : g.seg0;
         // queries: [dim / 8][row][dims 0 4 1 5 2 6 3 7]
         const T* q = static_cast<const T*>(a.q) + (long long)(q0 + j) * a.q_ts + (long long)head * a.q_hs;
-        const bool full = g.x == g.it.start && g.xe == g.it.end;
-        T* const dst = static_cast<T*>(a.out) + (long long)(q0 + j) * a.o_ts + (long long)head * a.o_hs;
-        float* const part = a.part + ((long long)blockIdx.x * 2 + (g.x > g.it.start ? 0 : 1)) * PR * (HD + 2);
-        const int pr = tile * 128 + row;
         if (!ok) {
-          not_done(live, full, dst, part, pr, q0 + j, head);
+          if (live) not_done(g, tile * 128 + row, q0 + j, head);
           return;
         }
         uint4 qv[HD / 8];
@@ -537,7 +536,11 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
         }
         if (ok && (ok = warp_wait(&ofull[tile][1], seg & 1))) {
           tc_after();
+          const bool full = g.x == g.it.start && g.xe == g.it.end;
           const float inv = l == 0.f ? 0.f : V_UP / l;
+          T* dst = static_cast<T*>(a.out) + (long long)(q0 + j) * a.o_ts + (long long)head * a.o_hs;
+          float* part = part_of(g);
+          const int pr = tile * 128 + row;
           #pragma unroll 1
           for (int c = 0; c < HD / 32; ++c) {
             uint32_t o[32];
@@ -562,8 +565,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
             part[PR * HD + pr] = m * a.scale_log2;
             part[PR * HD + PR + pr] = l;
           }
-        } else {
-          not_done(live, full, dst, part, pr, q0 + j, head);
+        } else if (live) {
+          not_done(g, tile * 128 + row, q0 + j, head);
         }
       }
     });
@@ -753,7 +756,6 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnArgs a, in
         __syncwarp();
       }
     });
-    else clear_rows<T, HD>(a, blockIdx.x * 2 + warp - 14, gridDim.x * 2);
   }
   __syncwarp();
   if (warp == 12 || warp == 13) {                           // every MMA has ended before the tensor memory goes back
@@ -789,7 +791,7 @@ cudaError_t launch_prompt(AttnArgs a, int n_sm, int spin, void* ws, cudaStream_t
   };
   kern<<<a.grid, THREADS, SMEM<HD>, s>>>(a, spin, vec(a.q, a.q_ts, a.q_hs), vec(a.out, a.o_ts, a.o_hs));
   e = cudaGetLastError();
-  return e == cudaSuccess ? launch_join<T, HD, PR>(a, 16, s) : e;
+  return e == cudaSuccess ? launch_join<T, HD, PR, true>(a, 16, s) : e;
 }
 
 #define BFP200_PROMPT(T) \
