@@ -393,7 +393,9 @@ typedef struct bfp200_kv4_attention_args {
  * (causal) and k > p - window (window > 0); one that sees none gives zeros and
  * -inf.  p is lens[s] - q_start[s + 1] + t as for the writing, also where that
  * or lens[s] lies past the table, of which the positions below max_pages * page
- * are seen; a token before the sequence (p < 0) or outside q_start sees none. */
+ * are seen; a token before the sequence (p < 0) or outside q_start sees none.
+ * Scores scale q.k up to 2^22 in magnitude are held apart; beyond that 32 bits
+ * do not resolve a weight, and a row may come out as NaN. */
 int bfp200_kv4_attention_dev(const bfp200_kv4_attention_args* args, void* stream);
 /* Bytes of workspace that the call needs: 0 without tokens or sequences, and
  * where max_pages * page is at most 128 (256 for HD <= 64) and the call is no

@@ -6,7 +6,8 @@
 // taken from a 32-bit table that the caller builds in 64 bits
 // (long-context scalings change only the table).  Products and sums are
 // single IEEE operations in 32 bits, rounded once to the output type; the
-// inverse (the gradient) negates s.  All three kernels are bound by memory.
+// inverse (the gradient) negates s.  rope and read are bound by memory; append
+// of prompts is not (figures at each kernel).
 #include "kv4.cuh"
 
 #include <cstring>
@@ -205,9 +206,10 @@ cudaError_t launch_rope(RopeArgs a, bool inter, cudaStream_t s) {
 // stay in registers over the rows, and the rows' loads are issued before the
 // token's place is looked up.  A row's nibbles go straight to their record: the
 // 4-byte (keys) and 2-byte (values) pieces of neighbouring tokens meet in L2.
-// 26.8k tokens of 32 / 8 heads of 128 float16: 155 us, 530 MB of DRAM traffic
-// (3.4 TB/s), 60% of the issue slots at 35% of the warps: instructions and the
-// loads' latency together.  Appending and reading back take 184 us so, 217
+// 26.8k tokens of 32 / 8 heads of 128 float16: 152 us, 531 MB of DRAM traffic
+// (3.5 TB/s), 60% of the issue slots at 35% of the warps, of whose stalls the
+// loads' latency is the largest part: neither instructions nor memory are at a
+// limit by themselves.  Appending and reading back take 180 us so, 217
 // before a pass held rows of one kind only, 207 at 2 CTAs an SM instead of 3 (more
 // registers a thread), 184 at 4 with half the rows in flight.
 // ---------------------------------------------------------------------------

@@ -25,16 +25,16 @@
 // accumulators are 32-bit.
 //
 // What bounds it.  The cache is read once (ncu: 321 MB for 320), but a
-// pair of cached values takes 5.5 thread instructions, most of them decoding: at
-// 64 sequences of up to 8191 positions, 32 / 8 heads of 128, 58% of the issue
-// slots and 53% of the ALU are taken while the cache comes at 3.7 TB/s (87 us; 49
+// pair of cached values takes 5.3 thread instructions, most of them decoding: at
+// 64 sequences of up to 8191 positions, 32 / 8 heads of 128, 57% of the issue
+// slots and 53% of the ALU are taken while the cache comes at 3.7 TB/s (86 us; 49
 // at the measured copy bandwidth), with 12 warps an SM.  Short or few sequences
 // are bound by the chain of one item (lengths, page, first block, joining): 256
-// sequences of up to 2047, 9 / 3 heads of 64, take 35 us where the bytes take 10;
+// sequences of up to 2047, 9 / 3 heads of 64, take 36 us where the bytes take 10;
 // a call for one sequence of 176 takes 14 us, launches included.
 //
 // Work split.  All (sequence, KV head, row tile) items are laid end to end in
-// blocks of 32 positions and cut evenly over the CTAs on the device, from the
+// blocks of 32 positions (64 at heads of 64 and fewer) and cut evenly over the CTAs on the device, from the
 // lengths there; cuts near an item's end move onto it.  Cut items leave
 // partial sums that a second, dependent launch joins in a fixed order.
 #include "kv4_attn.cuh"
@@ -148,7 +148,9 @@ struct Item {
   Seq q;
 };
 
-// What a CTA needs again behind an item's loop, which leaves no registers for it.
+// What a CTA needs again behind an item's loop, in shared memory meanwhile: the
+// loop has no registers left (64 sequences of up to 4000 positions, 32 / 8 heads of 64,
+// float32: 280 bytes of spills a thread and 55.8 us with it in registers, 8 and 49.3 so).
 struct Held {
   Item it;
   long long x, xe, x1;             // the CTA's blocks of the item, the end of its share
@@ -713,6 +715,7 @@ cudaError_t launch_attn(AttnArgs a, int n_sm, void* ws, cudaStream_t s) {
 // sequences of up to 4000 positions, 24 tokens of 32 / 8 heads: 82 us against 123),
 // at 64 and fewer dims, where decoding is half and the softmax all of the work,
 // from some 300 (100 tokens of 9 / 3 heads: 90 against 96; 48 tokens: 66 against 57).
+// Heads of 96 go with 128 and 32 with 64, unmeasured.
 // 32-bit queries would not fit its shared memory.
 int pick_nt(const Batch& b, int group, int hd, bool wide) {
   if (b.n_seq == 0) return 1;

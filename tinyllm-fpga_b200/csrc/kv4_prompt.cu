@@ -11,13 +11,14 @@
 // tensor core works for the other.
 //
 // What bounds it.  8192 tokens, 32 / 8 heads of 128, bfloat16, causal: 550 GFLOP
-// in 646 us, 851 TFLOP/s (51% of the measured matrix product).  A block of 128
+// in 657 us, 837 TFLOP/s (50% of the measured matrix product).  A block of 128
 // positions costs 2048 cycles of MMAs (64 each, measured alone) and 2048 of the
-// special function units (256 x 128 exponentials, 16 a cycle): both run at 42% to
-// 46%.  The rest is the chain of a row's softmax between two waits, and an item's
+// special function units (256 x 128 exponentials, 16 a cycle): both run at 41% to
+// 45%.  The rest is the chain of a row's softmax between two waits, and an item's
 // start and end.  With neither softmax nor decoding the first form took 715 us of
 // its 863: waits beside busy MMAs take some 300 cycles.  At heads of 64 the MMAs
-// are half and the softmax the same: 571 us.
+// are half and the softmax the same: 584 us.  binary16 (two operands of weights,
+// twice the output MMAs) takes 1023 us.
 // Tried: operands under the hardware's swizzle (decoding writes cost more
 // addresses: 925 us against 863); one warp for both tiles' MMAs (818 against 713
 // with one a tile); one lane polling the barriers for its warp (1075: slower).
