@@ -385,7 +385,7 @@ typedef struct bfp200_kv4_attention_args {
   void* workspace_dev;                    /* 16-byte aligned; contents do not matter */
   long long workspace_bytes;
   long long q_ts, q_hs, o_ts, o_hs;
-  long long H_Q, dtype, causal, window;   /* H_Q a multiple of H_KV; window 0: none */
+  long long H_Q, dtype, causal, window;   /* H_Q a multiple of H_KV, n_tokens * H_Q / H_KV below 2^31 - 512; window 0: none */
   double scale;
 } bfp200_kv4_attention_args;
 /* Softmax attention of the call's tokens over their sequences' cached

@@ -76,3 +76,20 @@ def test_no_exception_leaves_a_c_entry_point():
         with open(os.path.join(csrc, name)) as f:
             heads += re.findall(r'^extern "C" int (\w+)\([^)]*\) *(\w*)', f.read(), re.M)
     assert len(heads) >= 7 and [h for h, word in heads if word != "try"] == []
+
+
+@pytest.mark.parametrize("T,hq,H", [(1 << 20, 1 << 16, 1), (1 << 15, 1 << 16, 1), (1 << 28, 1 << 16, 1 << 10)])
+def test_attention_refuses_more_rows_than_it_counts(T, hq, H):
+    """The kernels count a KV head's rows, tokens times query heads, in 32 bits."""
+    from bfp200 import _lib, kv4
+    args = kv4._ATTENTION.pack(*_batch(T=T, H=H), *[4096] * 4, 1 << 40, *[64] * 4, hq, 0, 1, 0, 0.125)
+    for rc in (_lib.lib().bfp200_kv4_attention_dev(args, None), _lib.lib().bfp200_kv4_attention_workspace(args, _lib.C.c_size_t())):
+        assert rc == _lib.EINVAL and "rows" in _lib.last_error()
+
+
+def test_attention_workspace_checks_the_heads_as_attention_does():
+    from bfp200 import _lib, kv4
+    for hq in (0, 3, -2, (1 << 16) + 2, 1 << 33):
+        args = kv4._ATTENTION.pack(*_batch(), *[4096] * 4, 1 << 40, *[64] * 4, hq, 0, 1, 0, 0.125)
+        assert _lib.lib().bfp200_kv4_attention_dev(args, None) == _lib.EINVAL
+        assert _lib.lib().bfp200_kv4_attention_workspace(args, _lib.C.c_size_t()) == _lib.EINVAL

@@ -751,6 +751,14 @@ cudaError_t by_hd(int hd, const AttnArgs& a, int nt, int n_sm, int spin, void* w
                   : by_nt<T, 128>(a, nt, n_sm, spin, ws, s);
 }
 
+// What is wrong with a call's query heads, or null.  The kernels count the rows
+// of a KV head, and the items of a sequence, in 32 bits.
+const char* bad_heads(const Batch& b, long long HQ) {
+  if (HQ < 1 || HQ > (1LL << 16) || HQ % b.H) return "H_Q must be a positive multiple of H_KV";
+  if (b.T * (HQ / b.H) > (1LL << 31) - 512 || b.T * HQ > (1LL << 33)) return "too many rows (tokens times query heads)";
+  return nullptr;
+}
+
 // probe: a call of the prompts' kernel, whose waits give up at once
 int attention(const char* who, const bfp200_kv4_attention_args* in, bool probe, void* stream) {
   const auto bad = [&](const char* what) { return bfp200_set_error(BFP200_EINVAL, std::string(who) + ": " + what); };
@@ -760,7 +768,7 @@ int attention(const char* who, const bfp200_kv4_attention_args* in, bool probe, 
   if (int rc = fill_batch(r.batch, &a.b, who)) return rc;
   const int es = r.dtype == BFP200_F32 ? 4 : r.dtype == BFP200_F16 || r.dtype == BFP200_BF16 ? 2 : 0;
   if (!es) return bad("dtype must be BFP200_F32, BFP200_F16 or BFP200_BF16");
-  if (r.H_Q < 1 || r.H_Q > (1LL << 16) || r.H_Q % a.b.H) return bad("H_Q must be a positive multiple of H_KV");
+  if (const char* what = bad_heads(a.b, r.H_Q)) return bad(what);
   if (r.window < 0) return bad("window must not be negative");
   if (!(r.scale - r.scale == 0.0)) return bad("scale must be finite");
   if (a.b.T == 0) return BFP200_OK;
@@ -811,7 +819,7 @@ extern "C" int bfp200_kv4_attention_workspace(const bfp200_kv4_attention_args* i
   if (!in || !bytes) return bad("no arguments");
   Batch b;
   if (int rc = fill_batch(in->batch, &b, who)) return rc;
-  if (in->H_Q < 1 || in->H_Q % b.H) return bad("H_Q must be a positive multiple of H_KV");
+  if (const char* what = bad_heads(b, in->H_Q)) return bad(what);
   int n_sm = 0;
   if (int rc = device_ready(who, &n_sm)) return rc;
   const int hd = (int)in->batch.HD;
