@@ -329,3 +329,18 @@ def test_append_of_lowest_and_highest_mantissas(dtype):
     kv4.append(args[0], k, k, *args[1:])
     rk, rv = kv4.read(*args, 2, dtype=torch.float32)
     assert (rk[0] == -2.0).all() and (rk[1] == 1.75).all() and torch.equal(rk, rv)
+
+
+def test_check_done_waits_for_calls_without_a_workspace():
+    import torch
+    from bfp200 import kv4
+    case = Case(np.random.default_rng(0), [20], [1], 1, 64, 16)
+    q = torch.ones((1, 3, 64), device="cuda")
+    for t in (1, 0):
+        qs = _i32([0, t])
+        torch.cuda.synchronize()
+        torch.cuda._sleep(100_000_000)                       # some 50 ms
+        kv4.attention(q[:t], case.pool, qs, case.len_t, case.bt)
+        assert not torch.cuda.current_stream().query()
+        kv4.attention(q[:t], case.pool, qs, case.len_t, case.bt, check_done=True)
+        assert torch.cuda.current_stream().query()

@@ -319,6 +319,6 @@ def attention(q, pool, q_start, lens, block_table, scale=None, causal=True, wind
     _run(_fn("bfp200_kv4_attention_dev"),
          _ATTENTION.pack(*b, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, ws.data_ptr() if need else 0, need, qt, qh, ot, oh,
                          hq, code, causal, window, d ** -0.5 if scale is None else scale), dev)
-    if check_done and need:
-        _run(_fn("bfp200_kv4_attention_status"), ws.data_ptr(), dev)
+    if check_done:
+        _run(_fn("bfp200_kv4_attention_status"), ws.data_ptr() if need else None, dev)
     return (out, lse) if return_lse else out
